@@ -260,6 +260,86 @@ ONNXB200_API int onnxb200_nchw_to_nhwc(onnxb200_handle* h, int64_t n, int64_t c,
 ONNXB200_API int onnxb200_nhwc_to_nchw(onnxb200_handle* h, int64_t n, int64_t c, int64_t hh,
                                        int64_t ww, const float* x, float* y);
 
+/* ---------------------------------------------------------------- 8-bit linear path */
+/* Root-mean-square normalisation, block quantisation and the block-scaled matrix
+ * product of layers whose weights and activations are 8-bit floating point
+ * (e4m3: 4 exponent and 3 fraction bits, largest value 448, no infinity).  No
+ * counterpart in the reference (its tensors are fp32, src/ops/tensor.rs:206-218).
+ *
+ * A quantised matrix holds one byte per element and one fp32 scale for every
+ * block of 128 columns of a row (activations) or of 128 rows by 128 columns
+ * (weights); the last block of a row or column may be shorter.  An element
+ * stands for e4m3 * scale, with
+ *   amax = max(max |x| over the block, 2^-96),  scale = amax / 448,
+ *   e4m3 = nearest(x * (448 / amax)), ties to even, at most 448 in magnitude.
+ * A block that holds a NaN or an infinity gets a scale that is not finite: every
+ * element of it stands for NaN, and so does every product with it.
+ *
+ * Row strides (ld*) are in elements; 0 means dense.  Scales are addressed by two
+ * strides, in floats: scale of (row block i, column block j) at i * row + j *
+ * block; both 0 means dense rows.  Matrices and scales that are written must not
+ * overlap in themselves; elements between rows are never written.  An empty
+ * matrix is no error: nothing is done (a product with k = 0 writes the bias).
+ * These calls use no workspace: they may be captured into a CUDA graph, and
+ * graphs or handles that run at the same time share nothing. */
+#define ONNXB200_TYPE_F32 0
+#define ONNXB200_TYPE_F16 1
+#define ONNXB200_TYPE_BF16 2
+#define ONNXB200_TYPE_E4M3 3
+
+/* Columns of the longest row that onnxb200_rmsnorm takes. */
+#define ONNXB200_RMSNORM_MAX_COLS 49152
+
+typedef struct onnxb200_rmsnorm_desc {
+  int64_t rows, cols;
+  int64_t ldx, ldr, lds, ldy;          /* x, residual, sum, y */
+  int64_t y_scale_row, y_scale_block;  /* strides of y_scale (out_type E4M3) */
+  int type;                            /* of x, residual and sum: F32, F16 or BF16 */
+  int weight_type;                     /* F32, F16 or BF16 */
+  int out_type;                        /* of y: the same as `type`, or E4M3 */
+  float epsilon;                       /* >= 0 */
+} onnxb200_rmsnorm_desc;
+/* ONNX RMSNormalization (opset 23) over the last axis, with the addition in
+ * front of it and the quantisation behind it:
+ *   h = x + residual (residual may be NULL);  sum = h (may be NULL);
+ *   y = h / sqrt(mean(h^2) + epsilon) * weight.
+ * Everything between the loads and the stores is fp32: y is computed from the
+ * unrounded h, and rounded (or quantised, with y_scale) once.  sum and y may be
+ * the same memory as x or residual (same type and row stride). */
+ONNXB200_API int onnxb200_rmsnorm(onnxb200_handle* h, const onnxb200_rmsnorm_desc* d, const void* x,
+                                  const void* residual, const void* weight, void* sum, void* y,
+                                  float* y_scale);
+
+typedef struct onnxb200_quantize_desc {
+  int64_t rows, cols;
+  int64_t ldx, ldq;
+  int64_t scale_row, scale_block; /* strides of scale */
+  int type;                       /* of x: F32, F16 or BF16 */
+  int block_rows;                 /* 1 (activations) or 128 (weights) */
+} onnxb200_quantize_desc;
+/* Quantises x to e4m3 with one scale per block (formulas above). */
+ONNXB200_API int onnxb200_quantize_blocks(onnxb200_handle* h, const onnxb200_quantize_desc* d,
+                                          const void* x, void* q, float* scale);
+
+typedef struct onnxb200_matmul_blocks_desc {
+  int64_t m, n, k;
+  int64_t lda, ldb, ldy;
+  int64_t a_scale_row, a_scale_block; /* strides of a_scale, row = a row of a */
+  int64_t b_scale_row, b_scale_block; /* strides of b_scale, row = 128 rows of b */
+  int out_type;                       /* of y: F32, F16 or BF16 */
+  int flags;                          /* 0 or ONNXB200_EPI_RELU */
+} onnxb200_matmul_blocks_desc;
+/* y[m][n] = sum over blocks j of 128 k's of a_scale[m][j] * b_scale[n / 128][j] *
+ * sum_{k in j} a[m][k] * b[n][k], + bias[n] (fp32, may be NULL), Relu if asked;
+ * a is [m][k], b is [n][k], both e4m3.  The sums of a block are the tensor
+ * cores', over at most 128 products; blocks are scaled and added in fp32, and y
+ * is rounded once.  a and b on 16-byte boundaries with row strides that are
+ * multiples of 16 run on the tensor cores, others on the CUDA cores (slower,
+ * same formula). */
+ONNXB200_API int onnxb200_matmul_blocks(onnxb200_handle* h, const onnxb200_matmul_blocks_desc* d,
+                                        const void* a, const float* a_scale, const void* b,
+                                        const float* b_scale, const float* bias, void* y);
+
 /* ---------------------------------------------------------------- graphs */
 /* ONNX-style node list (the reference IR's Node, src/model.rs:162-172). */
 #define ONNXB200_ATTR_INT 0

@@ -34,6 +34,11 @@ pub const ONNXB200_COPY_H2D: c_int = 0;
 pub const ONNXB200_COPY_D2H: c_int = 1;
 pub const ONNXB200_COPY_D2D: c_int = 2;
 pub const ONNXB200_NOALLOC_SCRATCH_BYTES: usize = 25165824;
+pub const ONNXB200_TYPE_F32: c_int = 0;
+pub const ONNXB200_TYPE_F16: c_int = 1;
+pub const ONNXB200_TYPE_BF16: c_int = 2;
+pub const ONNXB200_TYPE_E4M3: c_int = 3;
+pub const ONNXB200_RMSNORM_MAX_COLS: c_int = 49152;
 pub const ONNXB200_ATTR_INT: c_int = 0;
 pub const ONNXB200_ATTR_FLOAT: c_int = 1;
 pub const ONNXB200_ATTR_INTS: c_int = 2;
@@ -124,6 +129,53 @@ pub struct ConvNdDesc {
     pub dilation: [i64; 3],
     pub auto_pad: c_int,
     pub relu: c_int,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct RmsnormDesc {
+    pub rows: i64,
+    pub cols: i64,
+    pub ldx: i64,
+    pub ldr: i64,
+    pub lds: i64,
+    pub ldy: i64,
+    pub y_scale_row: i64,
+    pub y_scale_block: i64,
+    pub type_: c_int,
+    pub weight_type: c_int,
+    pub out_type: c_int,
+    pub epsilon: f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct QuantizeDesc {
+    pub rows: i64,
+    pub cols: i64,
+    pub ldx: i64,
+    pub ldq: i64,
+    pub scale_row: i64,
+    pub scale_block: i64,
+    pub type_: c_int,
+    pub block_rows: c_int,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct MatmulBlocksDesc {
+    pub m: i64,
+    pub n: i64,
+    pub k: i64,
+    pub lda: i64,
+    pub ldb: i64,
+    pub ldy: i64,
+    pub a_scale_row: i64,
+    pub a_scale_block: i64,
+    pub b_scale_row: i64,
+    pub b_scale_block: i64,
+    pub out_type: c_int,
+    pub flags: c_int,
 }
 
 #[repr(C)]
@@ -238,6 +290,9 @@ extern "C" {
     pub fn onnxb200_batchnorm(h: *mut Handle, layout: c_int, n: i64, c: i64, hh: i64, ww: i64, x: *const f32, scale: *const f32, bias: *const f32, mean: *const f32, var: *const f32, epsilon: f32, y: *mut f32) -> c_int;
     pub fn onnxb200_nchw_to_nhwc(h: *mut Handle, n: i64, c: i64, hh: i64, ww: i64, c_pad: i64, x: *const f32, y: *mut f32) -> c_int;
     pub fn onnxb200_nhwc_to_nchw(h: *mut Handle, n: i64, c: i64, hh: i64, ww: i64, x: *const f32, y: *mut f32) -> c_int;
+    pub fn onnxb200_rmsnorm(h: *mut Handle, d: *const RmsnormDesc, x: *const c_void, residual: *const c_void, weight: *const c_void, sum: *mut c_void, y: *mut c_void, y_scale: *mut f32) -> c_int;
+    pub fn onnxb200_quantize_blocks(h: *mut Handle, d: *const QuantizeDesc, x: *const c_void, q: *mut c_void, scale: *mut f32) -> c_int;
+    pub fn onnxb200_matmul_blocks(h: *mut Handle, d: *const MatmulBlocksDesc, a: *const c_void, a_scale: *const f32, b: *const c_void, b_scale: *const f32, bias: *const f32, y: *mut c_void) -> c_int;
     pub fn onnxb200_graph_build(h: *mut Handle, nodes: *const Node, n_nodes: c_int, initializers: *const TensorInfo, n_init: c_int, inputs: *const TensorInfo, n_inputs: c_int, outputs: *const *const c_char, n_outputs: c_int, out: *mut *mut Graph) -> c_int;
     pub fn onnxb200_graph_run(h: *mut Handle, g: *mut Graph, inputs: *const *const f32, outputs: *const *mut f32) -> c_int;
     pub fn onnxb200_graph_run_host(h: *mut Handle, g: *mut Graph, inputs: *const *const f32, outputs: *const *mut f32) -> c_int;

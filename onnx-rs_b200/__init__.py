@@ -11,7 +11,8 @@ from .runtime import (Handle, OnnxB200Error, ValidationError, ExecutionError, Un
                       OperationTimeout, ResourceExhausted, InvalidGraph, InvalidOperator, IoError, ProtobufError,
                       InvalidModel)
 from .ops import (ExecutionContext, Operator, OperatorRegistry, Conv, ConvPlan, MatMul, Gemm, MaxPool,
-                  GlobalAveragePool, Relu, Add, BatchNormalization, Flatten)
+                  GlobalAveragePool, Relu, Add, BatchNormalization, Flatten,
+                  RMSNormalization, QuantizeBlocks, MatMulBlockScaled)
 from .graph import Graph, MultiGraph, infer_shapes
 from . import onnx_io, sharding, synth, workloads
 
@@ -21,4 +22,4 @@ __all__ = ["Handle", "OnnxB200Error", "ValidationError", "ExecutionError", "Unsu
            "OperationTimeout", "ResourceExhausted", "InvalidGraph", "InvalidOperator", "ExecutionContext",
            "Operator", "OperatorRegistry", "Conv", "ConvPlan", "MatMul", "Gemm", "MaxPool", "GlobalAveragePool", "Relu",
            "Add", "BatchNormalization", "Flatten", "Graph", "MultiGraph", "infer_shapes", "onnx_io", "synth", "workloads", "LIB_PATH",
-           "IoError", "ProtobufError", "InvalidModel"]
+           "IoError", "ProtobufError", "InvalidModel", "RMSNormalization", "QuantizeBlocks", "MatMulBlockScaled"]

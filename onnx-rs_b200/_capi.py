@@ -43,6 +43,9 @@ EPI_BN = 2
 EPI_RESIDUAL = 4
 EPI_RELU = 8
 
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_E4M3 = 0, 1, 2, 3
+RMSNORM_MAX_COLS = 49152
+
 ATTR_INT, ATTR_FLOAT, ATTR_INTS, ATTR_STRING = 0, 1, 2, 3
 
 
@@ -64,6 +67,24 @@ class ConvNdDesc(ctypes.Structure):
                 ("c_out", ctypes.c_int64), ("group", ctypes.c_int64)] + [
         (f, ctypes.c_int64 * 3) for f in ("in_", "kernel", "stride", "pad_begin", "pad_end", "dilation")] + [
         ("auto_pad", ctypes.c_int), ("relu", ctypes.c_int)]
+
+
+class RmsNormDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in
+                ("rows", "cols", "ldx", "ldr", "lds", "ldy", "y_scale_row", "y_scale_block")] + [
+        ("type", ctypes.c_int), ("weight_type", ctypes.c_int), ("out_type", ctypes.c_int),
+        ("epsilon", ctypes.c_float)]
+
+
+class QuantizeDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "cols", "ldx", "ldq", "scale_row", "scale_block")] + [
+        ("type", ctypes.c_int), ("block_rows", ctypes.c_int)]
+
+
+class MatmulBlocksDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in
+                ("m", "n", "k", "lda", "ldb", "ldy", "a_scale_row", "a_scale_block", "b_scale_row",
+                 "b_scale_block")] + [("out_type", ctypes.c_int), ("flags", ctypes.c_int)]
 
 
 class Attr(ctypes.Structure):
@@ -150,6 +171,9 @@ SIGNATURES = {
     "onnxb200_batchnorm": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _f32, _vp]),
     "onnxb200_nchw_to_nhwc": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
     "onnxb200_nhwc_to_nchw": (_int, [_vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "onnxb200_rmsnorm": (_int, [_vp, ctypes.POINTER(RmsNormDesc)] + [_vp] * 6),
+    "onnxb200_quantize_blocks": (_int, [_vp, ctypes.POINTER(QuantizeDesc)] + [_vp] * 3),
+    "onnxb200_matmul_blocks": (_int, [_vp, ctypes.POINTER(MatmulBlocksDesc)] + [_vp] * 6),
     "onnxb200_graph_build": (_int, [_vp, ctypes.POINTER(Node), _int, ctypes.POINTER(TensorInfo), _int,
                                     ctypes.POINTER(TensorInfo), _int, ctypes.POINTER(ctypes.c_char_p), _int,
                                     ctypes.POINTER(_vp)]),

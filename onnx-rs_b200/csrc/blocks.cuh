@@ -1,0 +1,63 @@
+// Device helpers of the 8-bit linear path: element loads and stores, e4m3
+// conversions and the scale of a block.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "blocks.h"
+
+namespace ob2 {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// max that keeps a NaN of either side (fmaxf drops it): a block that holds one
+// must not get a finite scale.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Scale of a block and the factor its elements are multiplied with, from its
+// largest magnitude.  The floor keeps the factor finite for an all-zero block;
+// the comparison is false for NaN, which therefore reaches both.
+__device__ __forceinline__ void block_scale(float amax, float& scale, float& inv) {
+  const float a = amax < kAmaxFloor ? kAmaxFloor : amax;
+  scale = __fdiv_rn(a, kE4m3Max);
+  inv = __fdiv_rn(kE4m3Max, a);
+}
+
+// fp32 -> e4m3, nearest even, saturating at 448; NaN stays NaN.
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+__device__ __forceinline__ float from_e4m3(uint8_t v) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+}
+
+// Calls f with a null pointer of the element type `t` (F32, F16 or BF16).
+template <typename F>
+auto with_type(int t, F f) {
+  if (t == kF32) return f((float*)nullptr);
+  if (t == kF16) return f((__half*)nullptr);
+  return f((__nv_bfloat16*)nullptr);
+}
+
+}  // namespace ob2

@@ -1,0 +1,57 @@
+// The 8-bit linear path: what its entry points (blocks_api.cu) and kernels
+// (norm_quant.cu, gemm_blocks.cu) share.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace ob2 {
+
+constexpr int kQBlock = 128;           // columns (and weight rows) of one scale
+constexpr float kE4m3Max = 448.f;
+constexpr float kAmaxFloor = 0x1p-96f;  // keeps 448 / amax finite
+
+// Element types, as ONNXB200_TYPE_*.
+enum ElemType { kF32 = 0, kF16 = 1, kBF16 = 2, kE4M3 = 3 };
+inline int elem_size(int t) { return t == kF32 ? 4 : t == kE4M3 ? 1 : 2; }
+
+struct RmsNormArgs {
+  const void* x;
+  const void* res;     // null: none
+  const void* weight;
+  void* sum;           // null: not wanted
+  void* y;
+  float* y_scale;      // out_type == kE4M3
+  int64_t rows;
+  int cols;
+  int64_t ldx, ldr, lds, ldy, ys_row, ys_block;
+  int type, weight_type, out_type;
+  float eps;
+};
+// Return a cudaError_t.
+int rmsnorm_launch(const RmsNormArgs& a, cudaStream_t stream);
+
+struct QuantizeArgs {
+  const void* x;
+  uint8_t* q;
+  float* scale;
+  int64_t rows, cols, ldx, ldq, s_row, s_block;
+  int type, block_rows;
+};
+int quantize_launch(const QuantizeArgs& a, cudaStream_t stream);
+
+struct MatmulBlocksArgs {
+  const uint8_t* a;
+  const uint8_t* b;
+  const float* as;
+  const float* bs;
+  const float* bias;   // null: none
+  void* y;
+  int m, n, k;
+  int64_t lda, ldb, ldy, as_row, as_block, bs_row, bs_block;
+  int out_type, relu;
+  int* status;         // device status word (ONNXB200_ERR_* on failure)
+};
+int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t stream);
+
+}  // namespace ob2

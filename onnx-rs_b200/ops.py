@@ -16,6 +16,7 @@ character codes instead, src/ops/registry.rs:105-106, and never matches).
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -503,6 +504,272 @@ class Flatten(Operator):
         return [x.reshape(self.output_shapes({"attrs": {"axis": self.axis}}, [list(x.shape)])[0])]
 
 
+# --------------------------------------------------------------------------- 8-bit linear path
+_TYPE = {torch.float32: C.TYPE_F32, torch.float16: C.TYPE_F16, torch.bfloat16: C.TYPE_BF16}
+_E4M3 = torch.float8_e4m3fn
+_ONNX_TYPE = {1: torch.float32, 10: torch.float16, 16: torch.bfloat16}  # TensorProto.DataType
+_QBLOCK = 128
+
+
+def _type(t, what):
+    code = _TYPE.get(t.dtype)
+    if code is None:
+        raise ValidationError(C.ERR_VALIDATION, f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _check_device(h, what, *tensors):
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != h.device):
+            raise ValidationError(C.ERR_VALIDATION, f"{what}: expected tensors on cuda:{h.device}, got {t.device}")
+
+
+def _row_stride(t, what):
+    """Row stride of a tensor read as the matrix [product of leading dims, last dim]."""
+    if t.dim() == 0:
+        raise ValidationError(C.ERR_VALIDATION, f"{what}: expected at least one dimension")
+    cols = t.shape[-1]
+    if t.numel() == 0 or t.is_contiguous():
+        return cols
+    stride = t.stride()
+    if cols > 1 and stride[-1] != 1:
+        raise ValidationError(C.ERR_VALIDATION, f"{what}: expected rows of consecutive elements")
+    ld = step = None
+    for size, st in zip(reversed(t.shape[:-1]), reversed(stride[:-1])):
+        if size == 1:
+            continue
+        if ld is None:
+            ld, step = st, st * size
+        elif st != step:
+            raise ValidationError(C.ERR_VALIDATION, f"{what}: the leading dimensions do not have one stride")
+        else:
+            step = st * size
+    if ld is None:
+        return cols
+    if ld < cols:
+        raise ValidationError(C.ERR_VALIDATION, f"{what}: the rows overlap")
+    return ld
+
+
+def _stored_rows(lead, cols, dev):
+    """Uninitialised e4m3 tensor [*lead, cols] whose rows start on 16-byte boundaries (what the
+    tensor-core product reads), with its row stride."""
+    ld = (cols + 15) // 16 * 16
+    if ld == cols:
+        return torch.empty((*lead, cols), dtype=_E4M3, device=dev), ld
+    return torch.empty((*lead, ld), dtype=_E4M3, device=dev)[..., :cols], ld
+
+
+def _stored_scales(lead, rows, blocks, dev):
+    """Uninitialised scales [*lead, blocks]; those of one block of columns lie side by side, as the
+    product reads them."""
+    s = torch.empty((blocks, rows), dtype=torch.float32, device=dev).t()
+    return s if len(lead) == 1 else s.unflatten(0, lead) if lead else s[0]
+
+
+def _scale_strides(s, rows, blocks, what):
+    """(tensor, row stride, block stride) of scales read as the matrix [rows, blocks]."""
+    if s.dtype != torch.float32:
+        raise ValidationError(C.ERR_VALIDATION, f"{what}: expected float32 scales, got {s.dtype}")
+    if s.dim() == 0 or s.shape[-1] != blocks or s.numel() != rows * blocks:
+        raise ValidationError(C.ERR_VALIDATION, f"{what}: expected {rows} x {blocks} scales, got {tuple(s.shape)}")
+    if s.dim() != 2:
+        s = s.reshape(rows, blocks)
+    sr, sb = s.stride()
+    if sr == 0 and sb == 0:  # one value for all: two zeros stand for dense rows at the C entry
+        s = s.contiguous()
+        sr, sb = s.stride()
+    return s, sr, sb
+
+
+def _launch(h, what, entry, desc, *args):
+    """Calls a C entry in order with torch's current stream, whatever stream the handle runs on."""
+    cur = torch.cuda.current_stream(h.device)
+    run = h.stream_ptr
+    side = None
+    # the handle's own stream is a blocking one: ordered with the legacy default stream by itself
+    if cur.cuda_stream != run and not (cur.cuda_stream == 0 and run == h.own_stream_ptr):
+        side = torch.cuda.ExternalStream(run, device=h.device)
+        side.wait_stream(cur)
+    rc = entry(h.ptr, ctypes.byref(desc), *args)
+    if side is not None:
+        cur.wait_stream(side)
+    if rc != 0:
+        h.check(rc, what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class RMSNormalization(Operator):
+    """ONNX RMSNormalization (opset 23) over the last axis.  Not in the reference registry.
+
+    compute([x, scale], ctx, residual=None) returns [y], or with ``quantize`` [q, q_scale]: e4m3
+    values and one fp32 scale for every 128 columns of a row, the operand form of
+    MatMulBlockScaled.  With a residual, h = x + residual is normalised and h (rounded to x's
+    type) is returned as the last output."""
+    op_type = "RMSNormalization"
+    min_inputs = 2
+
+    def __init__(self, epsilon=1e-5, axis=-1, quantize=False):
+        self.epsilon = float(epsilon)
+        self.axis = int(axis)
+        self.quantize = bool(quantize)
+
+    @classmethod
+    def from_node(cls, node, **kw):
+        a = _attrs(node)
+        return cls(a.get("epsilon", 1e-5), a.get("axis", -1), **kw)
+
+    def _check_axis(self, rank):
+        if self.axis not in (-1, rank - 1):
+            raise UnsupportedFeature(C.ERR_UNSUPPORTED, f"RMSNormalization: only the last axis, got {self.axis}")
+
+    def output_shapes(self, node, input_shapes):
+        x = input_shapes[0]
+        if x is not None:
+            type(self).from_node(node)._check_axis(len(x))
+        return [x]
+
+    def compute(self, inputs, ctx, residual=None):
+        x, w = inputs[0], inputs[1]
+        h = ctx.handle
+        what = "RMSNormalization"
+        _check_device(h, what, x, w, residual)
+        d = C.RmsNormDesc()
+        d.type = _type(x, what)
+        d.weight_type = _type(w, what)
+        d.ldx = _row_stride(x, what)
+        self._check_axis(x.dim())
+        lead, cols = tuple(x.shape[:-1]), x.shape[-1]
+        if w.dim() != 1 or w.shape[0] != cols or not w.is_contiguous():
+            raise ValidationError(C.ERR_VALIDATION, f"{what}: expected a contiguous scale of {cols} elements")
+        total = None
+        if residual is not None:
+            if residual.shape != x.shape or residual.dtype != x.dtype:
+                raise ValidationError(C.ERR_VALIDATION, f"{what}: the residual must have x's shape and type")
+            d.ldr = _row_stride(residual, what)
+            total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.rows, d.cols = math.prod(lead), cols
+        d.epsilon = self.epsilon
+        qs = None
+        if self.quantize:
+            d.out_type = C.TYPE_E4M3
+            blocks = (cols + _QBLOCK - 1) // _QBLOCK
+            y, d.ldy = _stored_rows(lead, cols, x.device)
+            qs = _stored_scales(lead, d.rows, blocks, x.device)
+            d.y_scale_row, d.y_scale_block = 1, max(1, d.rows)
+        else:
+            d.out_type = d.type
+            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _launch(h, what, C.lib().onnxb200_rmsnorm, d, _ptr(x), _ptr(residual), _ptr(w), _ptr(total), _ptr(y), _ptr(qs))
+        out = [y] if qs is None else [y, qs]
+        return out if total is None else out + [total]
+
+
+class QuantizeBlocks(Operator):
+    """e4m3 values and fp32 scales of a matrix: compute([x], ctx) returns [q, scale].  block_rows = 1
+    gives one scale for every 128 columns of a row (activations, any leading dims), block_rows = 128
+    one for 128 rows by 128 columns (weights, 2-D).  Not in the reference registry."""
+    op_type = "QuantizeBlocks"
+
+    def __init__(self, block_rows=1):
+        if block_rows not in (1, _QBLOCK):
+            raise ValidationError(C.ERR_VALIDATION, f"QuantizeBlocks: block_rows must be 1 or {_QBLOCK}, got {block_rows}")
+        self.block_rows = int(block_rows)
+
+    @classmethod
+    def from_node(cls, node, **kw):
+        return cls(_attrs(node).get("block_rows", 1), **kw)
+
+    def output_shapes(self, node, input_shapes):
+        x = input_shapes[0]
+        if x is None:
+            return [None, None]
+        br = type(self).from_node(node).block_rows
+        blocks = (x[-1] + _QBLOCK - 1) // _QBLOCK
+        return [list(x), list(x[:-1]) + [blocks] if br == 1 else [(x[0] + _QBLOCK - 1) // _QBLOCK, blocks]]
+
+    def compute(self, inputs, ctx):
+        x = inputs[0]
+        h = ctx.handle
+        what = "QuantizeBlocks"
+        _check_device(h, what, x)
+        d = C.QuantizeDesc()
+        d.type = _type(x, what)
+        d.ldx = _row_stride(x, what)
+        if self.block_rows != 1 and x.dim() != 2:
+            raise ValidationError(C.ERR_VALIDATION, f"{what}: weights must be 2-D")
+        lead, cols = tuple(x.shape[:-1]), x.shape[-1]
+        d.rows, d.cols = math.prod(lead), cols
+        d.block_rows = self.block_rows
+        blocks = (cols + _QBLOCK - 1) // _QBLOCK
+        q, d.ldq = _stored_rows(lead, cols, x.device)
+        if self.block_rows == 1:
+            s = _stored_scales(lead, d.rows, blocks, x.device)
+            d.scale_row, d.scale_block = 1, max(1, d.rows)
+        else:
+            s = torch.empty(((x.shape[0] + _QBLOCK - 1) // _QBLOCK, blocks), dtype=torch.float32, device=x.device)
+            d.scale_row, d.scale_block = max(1, blocks), 1
+        _launch(h, what, C.lib().onnxb200_quantize_blocks, d, _ptr(x), _ptr(q), _ptr(s))
+        return [q, s]
+
+
+class MatMulBlockScaled(Operator):
+    """y = A . B^T of e4m3 operands with a scale for every block of 128: compute([a, a_scale, b,
+    b_scale, bias?], ctx) returns [y].  a is [..., k] with a_scale [..., ceil(k / 128)], b is
+    [n, k] with b_scale [ceil(n / 128), ceil(k / 128)] (QuantizeBlocks(128)), bias fp32 [n]; y is
+    [..., n] in ``dtype``, after Relu if asked.  Not in the reference registry."""
+    op_type = "MatMulBlockScaled"
+    min_inputs = 4
+
+    def __init__(self, dtype=torch.float32, relu=False):
+        if dtype not in _TYPE:
+            raise ValidationError(C.ERR_VALIDATION,
+                                  f"MatMulBlockScaled: expected float32, float16 or bfloat16, got {dtype}")
+        self.dtype = dtype
+        self.relu = bool(relu)
+
+    @classmethod
+    def from_node(cls, node, **kw):
+        a = _attrs(node)
+        kw.setdefault("dtype", _ONNX_TYPE.get(a.get("dtype", 1)))
+        kw.setdefault("relu", a.get("relu", 0))
+        return cls(**kw)
+
+    def output_shapes(self, node, input_shapes):
+        a, b = input_shapes[0], input_shapes[2]
+        return [None if a is None or b is None else list(a[:-1]) + [b[0]]]
+
+    def compute(self, inputs, ctx):
+        a, a_scale, b, b_scale = inputs[:4]
+        bias = inputs[4] if len(inputs) > 4 else None
+        h = ctx.handle
+        what = "MatMulBlockScaled"
+        _check_device(h, what, a, a_scale, b, b_scale, bias)
+        if a.dtype != _E4M3 or b.dtype != _E4M3:
+            raise ValidationError(C.ERR_VALIDATION, f"{what}: expected float8_e4m3fn operands, got {a.dtype} and {b.dtype}")
+        d = C.MatmulBlocksDesc()
+        d.lda = _row_stride(a, what)
+        d.ldb = _row_stride(b, what)
+        if b.dim() != 2 or a.shape[-1] != b.shape[1]:
+            raise ValidationError(C.ERR_VALIDATION, f"Incompatible shapes for {what}: {list(a.shape)} and {list(b.shape)}")
+        n, k = b.shape
+        m = math.prod(a.shape[:-1])
+        blocks = (k + _QBLOCK - 1) // _QBLOCK
+        if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
+            raise ValidationError(C.ERR_VALIDATION, f"{what}: expected a contiguous float32 bias of {n} elements")
+        d.m, d.n, d.k = m, n, k
+        a_scale, d.a_scale_row, d.a_scale_block = _scale_strides(a_scale, m, blocks, what)
+        b_scale, d.b_scale_row, d.b_scale_block = _scale_strides(b_scale, (n + _QBLOCK - 1) // _QBLOCK, blocks, what)
+        d.out_type = _TYPE[self.dtype]
+        d.flags = C.EPI_RELU if self.relu else 0
+        y = torch.empty((*a.shape[:-1], n), dtype=self.dtype, device=a.device)
+        _launch(h, what, C.lib().onnxb200_matmul_blocks, d, _ptr(a), _ptr(a_scale), _ptr(b), _ptr(b_scale), _ptr(bias), _ptr(y))
+        return [y]
+
+
 # --------------------------------------------------------------------------- registry
 class OperatorRegistry:
     """(name, domain, version)-keyed registry (src/ops/registry.rs:30-128)."""
@@ -530,6 +797,10 @@ class OperatorRegistry:
                               ("Relu", 6, Relu), ("Add", 7, Add), ("BatchNormalization", 9, BatchNormalization),
                               ("Flatten", 9, Flatten)):
             r.register_operator(name, "", ver, op)
+        # the 8-bit linear path: RMSNormalization is ONNX's (opset 23), the others have no ONNX form
+        r.register_operator("RMSNormalization", "", 23, RMSNormalization)
+        r.register_operator("QuantizeBlocks", "b200", 1, QuantizeBlocks)
+        r.register_operator("MatMulBlockScaled", "b200", 1, MatMulBlockScaled)
         return r
 
     def create_operator_for_node(self, node, opset: int = 17, **kw) -> Operator:

@@ -97,6 +97,7 @@ class Handle:
             raise_for(rc, f"onnxb200_create(device={device}) failed: "
                           f"{self.lib.onnxb200_status_string(rc).decode()}")
         self.ptr = ptr
+        self.own_stream_ptr = self.stream_ptr
         if torch_stream:
             s = torch.cuda.current_stream(device)
             self.check(self.lib.onnxb200_set_stream(self.ptr, ctypes.c_void_p(s.cuda_stream)))

@@ -1,0 +1,200 @@
+"""CPU tests of the 8-bit linear path (RMSNormalization, QuantizeBlocks,
+MatMulBlockScaled): what the C entries and the operator classes refuse, the
+layouts the classes read and write, shapes and registration.  No kernel runs:
+the C entries check their arguments before they look at the (null) handle."""
+import ctypes
+
+import pytest
+import torch
+
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
+
+
+@pytest.fixture(scope="module")
+def C(ob):
+    return ob._capi
+
+
+def norm_desc(C, **kw):
+    d = C.RmsNormDesc(rows=4, cols=256, type=BF16, weight_type=BF16, out_type=BF16, epsilon=1e-5)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def quant_desc(C, **kw):
+    d = C.QuantizeDesc(rows=4, cols=256, type=BF16, block_rows=1)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def mm_desc(C, **kw):
+    d = C.MatmulBlocksDesc(m=4, n=256, k=256, out_type=F32)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+P = ctypes.c_void_p(4096)  # never read
+
+
+def call_norm(C, d, x=P, res=None, w=P, s=None, y=P, ys=P):
+    return C.lib().onnxb200_rmsnorm(None, ctypes.byref(d) if d else None, x, res, w, s, y, ys)
+
+
+def call_quant(C, d, x=P, q=P, s=P):
+    return C.lib().onnxb200_quantize_blocks(None, ctypes.byref(d) if d else None, x, q, s)
+
+
+def call_mm(C, d, a=P, sa=P, b=P, sb=P, bias=None, y=P):
+    return C.lib().onnxb200_matmul_blocks(None, ctypes.byref(d) if d else None, a, sa, b, sb, bias, y)
+
+
+def test_valid_arguments_reach_the_handle_check(C):
+    odd = ctypes.c_void_p(4097)
+    for rc in (call_norm(C, norm_desc(C)), call_norm(C, norm_desc(C, out_type=E4M3)), call_quant(C, quant_desc(C)),
+               call_quant(C, quant_desc(C, block_rows=128)), call_mm(C, mm_desc(C)), call_mm(C, mm_desc(C, k=0), None, None, None, None),
+               call_norm(C, norm_desc(C, rows=0), None, None, None, None, None, None),
+               call_quant(C, quant_desc(C, cols=0), None, None, None), call_mm(C, mm_desc(C, m=0), None, None, None, None),
+               call_mm(C, mm_desc(C, a_scale_row=0, a_scale_block=1)),  # one row of scales for all rows of a
+               call_mm(C, mm_desc(C, lda=257), a=odd),                  # bytes have no alignment of their own
+               call_norm(C, norm_desc(C, cols=C.RMSNORM_MAX_COLS))):
+        assert rc == C.ERR_INVALID_ARGUMENT
+    # the null descriptor and the null handle give the same code; the others below do not
+    assert call_norm(C, None) == call_quant(C, None) == call_mm(C, None) == C.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("kw", [
+    {"type": E4M3}, {"type": 7}, {"type": -1}, {"weight_type": E4M3}, {"out_type": F32}, {"out_type": F16},
+    {"rows": -1}, {"rows": 1 << 31}, {"cols": 0}, {"cols": -5}, {"epsilon": -1.0}, {"epsilon": float("nan")},
+    {"ldx": 255}, {"ldr": 1}, {"lds": -256}, {"ldy": 128}, {"ldx": 1 << 40},
+    {"out_type": E4M3, "y_scale_row": 1, "y_scale_block": 1}, {"out_type": E4M3, "y_scale_row": 1, "y_scale_block": 3},
+    {"out_type": E4M3, "y_scale_row": 0, "y_scale_block": 1}, {"out_type": E4M3, "y_scale_row": -2, "y_scale_block": 1},
+])
+def test_rmsnorm_refuses(C, kw):
+    assert call_norm(C, norm_desc(C, **kw)) == C.ERR_VALIDATION
+
+
+def test_rmsnorm_refuses_long_rows_and_bad_pointers(C):
+    assert call_norm(C, norm_desc(C, cols=C.RMSNORM_MAX_COLS + 1)) == C.ERR_UNSUPPORTED
+    odd = ctypes.c_void_p(4097)
+    assert call_norm(C, norm_desc(C), x=odd) == C.ERR_VALIDATION
+    assert call_norm(C, norm_desc(C), res=odd) == C.ERR_VALIDATION
+    assert call_norm(C, norm_desc(C), s=odd) == C.ERR_VALIDATION
+    assert call_norm(C, norm_desc(C), w=odd) == C.ERR_VALIDATION
+    assert call_norm(C, norm_desc(C), y=odd) == C.ERR_VALIDATION
+    assert call_norm(C, norm_desc(C, out_type=E4M3), y=odd, ys=odd) == C.ERR_VALIDATION
+
+
+@pytest.mark.parametrize("kw", [
+    {"type": E4M3}, {"type": 9}, {"block_rows": 0}, {"block_rows": 64}, {"rows": -1}, {"cols": -1}, {"cols": 1 << 31},
+    {"ldx": 255}, {"ldq": 17}, {"scale_row": 1, "scale_block": 1}, {"scale_row": 1, "scale_block": 0},
+    {"rows": 300, "block_rows": 128, "scale_row": 1, "scale_block": 2},
+])
+def test_quantize_refuses(C, kw):
+    assert call_quant(C, quant_desc(C, **kw)) == C.ERR_VALIDATION
+
+
+def test_quantize_refuses_too_many_blocks_and_bad_pointers(C):
+    assert call_quant(C, quant_desc(C, rows=1 << 30, cols=1024)) == C.ERR_UNSUPPORTED
+    assert call_quant(C, quant_desc(C), x=ctypes.c_void_p(4097)) == C.ERR_VALIDATION
+    assert call_quant(C, quant_desc(C), s=ctypes.c_void_p(4098)) == C.ERR_VALIDATION
+
+
+@pytest.mark.parametrize("kw", [
+    {"out_type": E4M3}, {"out_type": 4}, {"flags": 1}, {"flags": 16}, {"m": -1}, {"n": -1}, {"k": -1}, {"m": 1 << 31},
+    {"lda": 255}, {"ldb": -1}, {"ldy": 100}, {"a_scale_row": -1, "a_scale_block": 1}, {"b_scale_row": 1, "b_scale_block": -1},
+])
+def test_matmul_refuses(C, kw):
+    assert call_mm(C, mm_desc(C, **kw)) == C.ERR_VALIDATION
+
+
+def test_matmul_refuses_too_many_tiles_and_bad_pointers(C):
+    assert call_mm(C, mm_desc(C, m=1 << 30, n=1 << 30)) == C.ERR_UNSUPPORTED
+    odd = ctypes.c_void_p(4097)
+    assert call_mm(C, mm_desc(C), sa=odd) == call_mm(C, mm_desc(C), sb=odd) == C.ERR_VALIDATION
+    assert call_mm(C, mm_desc(C), bias=odd) == call_mm(C, mm_desc(C), y=odd) == C.ERR_VALIDATION
+
+
+def test_row_stride(ob):
+    stride = ob.ops._row_stride
+    x = torch.zeros(6, 40)
+    assert stride(x, "x") == 40
+    assert stride(x[:, :33], "x") == 40
+    assert stride(x[::2, :33], "x") == 80
+    assert stride(torch.zeros(2, 3, 40)[:, :, :7], "x") == 40
+    assert stride(torch.zeros(5), "x") == 5
+    assert stride(torch.zeros(5, 0), "x") == 0
+    assert stride(torch.zeros(4, 1)[::2], "x") == 2
+    assert stride(x[:1, :33], "x") == 33  # a single row has no stride
+    for bad in (x.t(), x[:, ::2], torch.zeros(2, 3, 40)[:, :2], torch.zeros(1, 40).expand(6, 40), torch.zeros(())):
+        with pytest.raises(ob.ValidationError):
+            stride(bad, "x")
+
+
+def test_stored_layouts(ob):
+    q, ld = ob.ops._stored_rows((3, 2), 33, "cpu")
+    assert q.shape == (3, 2, 33) and ld == 48 and ob.ops._row_stride(q, "q") == 48
+    q, ld = ob.ops._stored_rows((), 64, "cpu")
+    assert q.shape == (64,) and ld == 64
+    for lead, rows in (((3, 2), 6), ((6,), 6), ((), 1), ((1,), 1)):
+        s = ob.ops._stored_scales(lead, rows, 5, "cpu")
+        assert s.shape == (*lead, 5)
+        back, sr, sb = ob.ops._scale_strides(s, rows, 5, "s")
+        assert back.data_ptr() == s.data_ptr()  # read in place, never copied
+        assert (rows == 1 or sr == 1) and sb == rows
+
+
+def test_scale_strides(ob):
+    f = ob.ops._scale_strides
+    one = torch.ones(1, 1).expand(4, 3)  # one value for all: laid out densely
+    s, sr, sb = f(one, 4, 3, "s")
+    assert (sr, sb) == (3, 1) and s.is_contiguous()
+    row = torch.ones(1, 3).expand(4, 3)  # one row for all rows: read as it is
+    s, sr, sb = f(row, 4, 3, "s")
+    assert (sr, sb) == (0, 1)
+    for bad in (torch.ones(4, 4), torch.ones(3, 3), torch.ones(4, 3).double(), torch.tensor(1.0)):
+        with pytest.raises(ob.ValidationError):
+            f(bad, 4, 3, "s")
+
+
+def test_operators_refuse_host_tensors_and_bad_arguments(ob):
+    class NoGpu:
+        device = 0
+    ctx = ob.ExecutionContext(NoGpu())
+    x = torch.zeros(2, 128)
+    for call in (lambda: ob.RMSNormalization().compute([x, x[0]], ctx), lambda: ob.QuantizeBlocks().compute([x], ctx),
+                 lambda: ob.MatMulBlockScaled().compute([x, x, x, x], ctx)):
+        with pytest.raises(ob.ValidationError, match="expected tensors on cuda:0"):
+            call()
+    with pytest.raises(ob.ValidationError):
+        ob.QuantizeBlocks(block_rows=64)
+    with pytest.raises(ob.ValidationError):
+        ob.MatMulBlockScaled(dtype=torch.float64)
+    with pytest.raises(ob.UnsupportedFeature):
+        ob.RMSNormalization(axis=1).output_shapes({"attrs": {"axis": 1}}, [[2, 3, 4]])
+
+
+def test_registry_and_shapes(ob):
+    r = ob.OperatorRegistry.initialize_standard_operators()
+    node = {"op": "RMSNormalization", "inputs": ["x", "w"], "outputs": ["y"], "attrs": {"epsilon": 1e-6, "axis": -1}}
+    op = r.create_operator_for_node(node, opset=23)
+    assert isinstance(op, ob.RMSNormalization) and op.epsilon == 1e-6
+    op.validate(node)
+    assert op.output_shapes(node, [[2, 3, 128], [128]]) == [[2, 3, 128]]
+    with pytest.raises(ob.InvalidOperator):  # not in the opset before 23
+        r.create_operator_for_node(node, opset=22)
+    qn = {"op": "QuantizeBlocks", "domain": "b200", "inputs": ["x"], "outputs": ["q", "s"], "attrs": {"block_rows": 128}}
+    assert r.create_operator_for_node(qn).output_shapes(qn, [[300, 130]]) == [[300, 130], [3, 2]]
+    qn["attrs"] = {}
+    assert r.create_operator_for_node(qn).output_shapes(qn, [[4, 300, 130]]) == [[4, 300, 130], [4, 300, 2]]
+    mn = {"op": "MatMulBlockScaled", "domain": "b200", "inputs": ["a", "as", "b", "bs"], "outputs": ["y"],
+          "attrs": {"dtype": 16, "relu": 1}}
+    mm = r.create_operator_for_node(mn)
+    assert mm.dtype == torch.bfloat16 and mm.relu
+    assert mm.output_shapes(mn, [[2, 5, 64], None, [100, 64], None]) == [[2, 5, 100]]
+    with pytest.raises(ob.ValidationError):
+        mm.validate({"inputs": ["a", "as", "b"], "outputs": ["y"]})
+    with pytest.raises(ob.ValidationError):
+        r.create_operator_for_node({**mn, "attrs": {"dtype": 7}})
