@@ -1,11 +1,24 @@
-// Block-scaled matrix product of e4m3 operands.
+// Block-scaled matrix product of e4m3 operands,
+//   y[m][n] = sum_j sa[m][j] * sb[n / 128][j] * sum_{k in block j} a[m][k] b[n][k] + bias[n].
+//
+// The scales change every 128 k's, so a block's sum leaves the tensor core before
+// the next one is added: each block of 128 k's is one accumulation in TMEM, which
+// the epilogue warps read, scale and add to a running total in fp32 registers
+// while the tensor core works on the next block in another TMEM buffer.
+#include <cuda.h>
+
+#include <algorithm>
+
 #include "blocks.cuh"
+#include "ptx.cuh"
 
 namespace ob2 {
 namespace {
 
-// CUDA cores: 64 x 64 outputs per block, 4 x 4 per thread; the products of a
-// block of 128 k's are summed in fp32, then scaled and added to the total.
+// ---------------------------------------------------------------- CUDA cores
+// Operands that TMA cannot read (row strides or pointers off the 16-byte grid):
+// 64 x 64 outputs per block, 4 x 4 per thread; the products of a block of 128
+// k's are summed in fp32, then scaled and added to the total.
 template <typename T>
 __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlocksArgs p) {
   __shared__ float sa[32][65], sb[32][65];
@@ -57,14 +70,597 @@ __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlo
     }
 }
 
+// ---------------------------------------------------------------- few rows
+// Tokens are the MMA's N and weights its M: a tile is 128 rows of b by BN rows of
+// a, so a handful of tokens wastes no tensor-core rows and y's columns (n) lie
+// along the lanes, whose stores are then contiguous.  The k range is split over
+// the CTAs of a cluster; each leaves its partial sums in shared memory, and the
+// sums are joined in rank order over distributed shared memory: one launch, no
+// workspace, the same bits every time.
+template <int BN>
+struct RowsLayout {
+  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
+  static constexpr int kW = 128 * 128, kX = BN * 128, kStage = kW + kX;
+  static constexpr int kBufs = BN == 128 ? 2 : 4;          // TMEM accumulators
+  static constexpr int kCols = BN * kBufs;                  // 64, 128, 256, 256
+  static constexpr int kChunk = 1024 / BN;                  // k-blocks whose scales are staged at once
+  static constexpr int kOffScale = kStages * kStage;        // 2 x kChunk x BN floats
+  static constexpr int kOffBar = kOffScale + 2 * 4096;
+  static constexpr int kBars = 2 * kStages + 2 * kBufs + 1;
+  static constexpr int kOffMisc = kOffBar + 8 * kBars;
+  static constexpr int kBytes = kOffMisc + 16 + 1024;       // base rounded up to 1024
+  static_assert(BN * 128 * 4 <= kStages * kStage, "partial sums reuse the stages");
+};
+constexpr int kRowsThreads = 192;  // 4 epilogue warps, TMA, MMA
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kRowsThreads, 2)
+    matmul_blocks_rows_kernel(const __grid_constant__ MatmulBlocksArgs p, const __grid_constant__ CUtensorMap tm_w,
+                              const __grid_constant__ CUtensorMap tm_x, int split, int x_tiles) {
+  using L = RowsLayout<BN>;
+  constexpr int ST = L::kStages, NB = L::kBufs, CH = L::kChunk;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t bar0 = base + L::kOffBar;
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * ST + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * ST + NB + b); };
+  const uint32_t drain = bar0 + 8u * (2 * ST + 2 * NB);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + L::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(smem_u32(tmem_slot), L::kCols);
+    tmem_relinquish();
+  }
+  if (warp == 4 && lane == 0) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int rank = blockIdx.x % split;
+  const int tile = blockIdx.x / split;
+  const int n0 = tile / x_tiles * 128, m0 = tile % x_tiles * BN;
+  const int kbs = (p.k + kQBlock - 1) / kQBlock;
+  const int kb0 = (int)((int64_t)kbs * rank / split), kb1 = (int)((int64_t)kbs * (rank + 1) / split);
+  const int nkb = kb1 - kb0;
+
+  float acc[BN];  // epilogue threads: row n0 + threadIdx.x, one column per token
+  if (warp < 4) {
+#pragma unroll
+    for (int j = 0; j < BN; ++j) acc[j] = 0.f;
+    // Scales of CH k-blocks at a time, sa * sb, 8 values per thread: loaded a
+    // chunk ahead into registers, shared through one of two buffers.
+    float* sc = reinterpret_cast<float*>(gbase + L::kOffScale);
+    const float* bs = p.bs + (n0 / kQBlock) * p.bs_row;
+    float nxt[8];
+    auto load_scales = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int idx = i * 128 + threadIdx.x;
+        const int kb = kb0 + c * CH + idx / BN, m = m0 + idx % BN;
+        nxt[i] = kb < kb1 && m < p.m ? p.as[m * p.as_row + kb * p.as_block] * bs[kb * p.bs_block] : 0.f;
+      }
+    };
+    load_scales(0);
+    bool ok = true;
+    const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    for (int it = 0; it < nkb; ++it) {
+      const int c = it / CH;
+      float* buf = sc + (c & 1) * 1024;
+      if (it % CH == 0) {
+        // the buffer's readers of chunk c - 2 passed the barrier of chunk c - 1
+#pragma unroll
+        for (int i = 0; i < 8; ++i) buf[i * 128 + threadIdx.x] = nxt[i];
+        ok = named_bar_and(ok, 128);
+        if ((c + 1) * CH < nkb) load_scales(c + 1);
+      }
+      // after a wait that gave up, the warp only keeps the barriers above going
+      const int b = it % NB;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full(b), (it / NB) & 1, abort_flag, p.status));
+      if (!ok) continue;
+      tc_fence_after();
+      const float4* s4 = reinterpret_cast<const float4*>(buf + it % CH * BN);
+#pragma unroll
+      for (int g = 0; g < BN / 16; ++g) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(lane_addr + b * BN + g * 16, r);
+        tmem_ld_wait();
+        if (g == BN / 16 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty(b));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 s = s4[g * 4 + q];
+          float* a = acc + g * 16 + q * 4;
+          a[0] = fmaf(__uint_as_float(r[q * 4]), s.x, a[0]);
+          a[1] = fmaf(__uint_as_float(r[q * 4 + 1]), s.y, a[1]);
+          a[2] = fmaf(__uint_as_float(r[q * 4 + 2]), s.z, a[2]);
+          a[3] = fmaf(__uint_as_float(r[q * 4 + 3]), s.w, a[3]);
+        }
+      }
+    }
+  } else if (warp == 4) {
+    if (lane == 0) {
+      int it = 0;
+      for (; it < nkb; ++it) {
+        const int s = it % ST;
+        if (!mbar_wait(empty(s), ((it / ST) & 1) ^ 1, abort_flag, p.status)) break;
+        mbar_arrive_expect_tx(full(s), L::kStage);
+        const uint32_t dst = base + s * L::kStage;
+        tma_load_2d(dst, &tm_w, (kb0 + it) * kQBlock, n0, full(s));
+        tma_load_2d(dst + L::kW, &tm_x, (kb0 + it) * kQBlock, m0, full(s));
+      }
+      // every copy has landed before the CTA may exit
+      volatile int no_abort = 0;
+      for (int i = max(0, it - ST); i < it; ++i) mbar_wait(full(i % ST), (i / ST) & 1, &no_abort, p.status);
+    }
+    __syncwarp();
+  } else {
+    constexpr uint32_t idesc = make_idesc(0, 128, BN);
+    if (lane == 0) {
+      int it = 0;
+      for (; it < nkb; ++it) {
+        const int s = it % ST, b = it % NB;
+        if (!mbar_wait(acc_empty(b), ((it / NB) & 1) ^ 1, abort_flag, p.status)) break;
+        if (!mbar_wait(full(s), (it / ST) & 1, abort_flag, p.status)) break;
+        tc_fence_after();
+        const uint64_t dw = smem_desc_sw128(base + s * L::kStage);
+        const uint64_t dx = smem_desc_sw128(base + s * L::kStage + L::kW);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma_e4m3<1>(tmem + b * BN, dw + (uint64_t)(kk * 2), dx + (uint64_t)(kk * 2), idesc, kk ? 1u : 0u);
+        tc_commit(empty(s));
+        tc_commit(acc_full(b));
+      }
+      if (it) {  // every MMA has completed before TMEM is freed
+        tc_commit(drain);
+        volatile int no_abort = 0;
+        mbar_wait(drain, 0, &no_abort, p.status);
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kCols);
+  }
+
+  T* y = static_cast<T*>(p.y);
+  const int n = n0 + (threadIdx.x & 127);
+  auto finish = [&](int j, float v, float bias) {
+    const int m = m0 + j;
+    if (m < p.m && n < p.n) {
+      v += bias;
+      if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays NaN
+      y[m * p.ldy + n] = from_f32<T>(v);
+    }
+  };
+  const float bias = warp < 4 && p.bias && n < p.n ? p.bias[n] : 0.f;
+  if (split == 1) {
+    if (warp < 4) {
+#pragma unroll
+      for (int j = 0; j < BN; ++j) finish(j, acc[j], bias);
+    }
+    return;
+  }
+  // partial[j][row] in the stages, which every MMA and copy has left
+  float* part = reinterpret_cast<float*>(gbase);
+  if (warp < 4) {
+#pragma unroll
+    for (int j = 0; j < BN; ++j) part[j * 128 + threadIdx.x] = acc[j];
+  }
+  cluster_sync();
+  if (warp < 4) {
+    const int j0 = BN * rank / split, j1 = BN * (rank + 1) / split;
+    const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
+    for (int j = j0; j < j1; ++j) {
+      float v = 0.f;
+      for (int q = 0; q < split; ++q) v += ld_cluster_f32(map_to_rank(mine + j * 512, q));
+      finish(j, v, bias);
+    }
+  }
+  cluster_sync();  // no CTA leaves while another reads its partial sums
+}
+
+// ---------------------------------------------------------------- many rows
+// A pair of CTAs computes 256 rows of a by BN rows of b (cta_group::2: each CTA
+// loads its 128 rows of a and half of the rows of b, and holds its 128 rows of
+// the accumulator).  Warps 0-7 of each CTA keep the running totals, thread =
+// row of y, BN / 2 columns each; a row's scale is then one register and the
+// weights' scale the same for all of a warp's columns.  Persistent: pairs walk
+// the tiles, and the next tile's loads and MMAs run during a tile's stores.
+template <int BN>
+struct PairLayout {
+  static constexpr int kA = 128 * 128, kB = BN / 2 * 128, kStage = kA + kB;
+  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kOut = 8 * 4096;                // per epilogue warp: 32 rows of 128 bytes
+  static constexpr int kOffOut = kStages * kStage;
+  static constexpr int kOffBar = kOffOut + kOut;
+  static constexpr int kBars = 2 * kStages + 5;
+  static constexpr int kOffMisc = kOffBar + 8 * kBars;
+  static constexpr int kBytes = kOffMisc + 16 + 1024;
+  static constexpr int kCols = 2 * BN;                 // two TMEM accumulators
+  static constexpr int kCW = BN / 2;                   // columns per epilogue warp
+};
+// 8 epilogue warps, then a warpgroup with the TMA and the MMA warp.  Launched with
+// 168 registers a thread (3 x 128 x 168 = 64512), split as 208 for the totals and 88
+// for the rest (2 x 128 x 208 + 128 x 88 = 64512).
+constexpr int kPairThreads = 384;
+constexpr int kGroupM = 8;         // tile order: columns of 8 tiles, so that pairs running together share operands
+
+template <typename T, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    matmul_blocks_pair_kernel(const __grid_constant__ MatmulBlocksArgs p, const __grid_constant__ CUtensorMap tm_a,
+                              const __grid_constant__ CUtensorMap tm_b) {
+  using L = PairLayout<BN>;
+  constexpr int ST = L::kStages, CW = L::kCW;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t bar0 = base + L::kOffBar;
+  auto full = [&](int s) { return bar0 + 8u * s; };           // leader's: both CTAs' bytes
+  auto empty = [&](int s) { return bar0 + 8u * (ST + s); };   // own
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * ST + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * ST + 2 + b); };  // leader's: 16 warps
+  const uint32_t drain = bar0 + 8u * (2 * ST + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + L::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 16);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 9) tmem_alloc_pair(smem_u32(tmem_slot), L::kCols);
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int tm = (p.m + 255) / 256, tn = (p.n + BN - 1) / BN;
+  const int tiles = tm * tn, pairs = gridDim.x / 2;
+  const int nkb = (p.k + kQBlock - 1) / kQBlock;
+  auto tile_at = [&](int t, int& mt, int& nt) {
+    const int per = kGroupM * tn, g = t / per, rem = t - g * per;
+    const int rows = min(kGroupM, tm - g * kGroupM);
+    mt = g * kGroupM + rem % rows;
+    nt = rem / rows;
+  };
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int sub = warp & 3, half = warp >> 2;
+    const uint32_t lane_addr = tmem + ((uint32_t)(sub * 32) << 16) + half * CW;
+    const uint32_t remote_empty0 = map_to_rank(acc_empty(0), 0), remote_empty1 = map_to_rank(acc_empty(1), 0);
+    const uint32_t out = base + L::kOffOut + warp * 4096;
+    constexpr int ES = sizeof(T), CPR = 128 / ES;  // columns per 128-byte staging row
+    const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.ldy * ES % 16 == 0;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
+      const int col0 = nt * BN + half * CW;
+      const int row = row0 + lane;
+      const float* as = p.as + (int64_t)min(row, p.m - 1) * p.as_row;
+      const float* bs = p.bs + (int64_t)(min(col0, p.n - 1) / kQBlock) * p.bs_row;
+      uint64_t acc[CW / 2];
+#pragma unroll
+      for (int j = 0; j < CW / 2; ++j) acc[j] = 0;
+      float na[4], nb[4];  // the next four blocks' scales
+      auto load_scales = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = min(kb + i, nkb - 1);
+          na[i] = as[k * p.as_block];
+          nb[i] = bs[k * p.bs_block];
+        }
+      };
+      load_scales(0);
+      for (int kb = 0; kb < nkb && ok; kb += 4) {
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = na[i] * nb[i];
+        if (kb + 4 < nkb) load_scales(kb + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (kb + i >= nkb) break;
+          const int b = it & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), (it >> 1) & 1, abort_flag, p.status));
+          if (!ok) break;
+          ++it;
+          tc_fence_after();
+          const uint64_t s2 = pack_f2(s[i], s[i]);
+          const uint32_t src = lane_addr + b * BN;
+          uint32_t r[2][16];
+          tmem_ld_32x32b_x16(src, r[0]);
+#pragma unroll
+          for (int g = 0; g < CW / 16; ++g) {
+            tmem_ld_wait();
+            if (g + 1 < CW / 16) {
+              tmem_ld_32x32b_x16(src + (g + 1) * 16, r[(g + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(b ? remote_empty1 : remote_empty0);
+            }
+            const uint32_t* q = r[g & 1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              acc[g * 8 + j] = fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2, acc[g * 8 + j]);
+          }
+        }
+      }
+      if (!ok) break;
+      // Bias, Relu, rounding; then through shared memory (16-byte units XORed
+      // with the row, free of bank conflicts both ways) so that a warp's stores
+      // are whole 128-byte lines of four rows at a time.
+#pragma unroll
+      for (int c = 0; c < CW / CPR; ++c) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          uint32_t w[4];
+          T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+          for (int q = 0; q < 16 / ES; ++q) {
+            const int j = c * CPR + u * (16 / ES) + q;
+            const float2 f = unpack_f2(acc[j / 2]);
+            float v = j & 1 ? f.y : f.x;
+            if (p.bias && col0 + j < p.n) v += p.bias[col0 + j];
+            if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays NaN
+            e[q] = from_f32<T>(v);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((u ^ (lane & 7)) * 16)), "r"(w[0]),
+                       "r"(w[1]), "r"(w[2]), "r"(w[3])
+                       : "memory");
+        }
+        __syncwarp();
+        const int u = lane & 7, col = col0 + c * CPR + u * (16 / ES);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int rr = q * 4 + (lane >> 3);
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(out + rr * 128 + ((u ^ (rr & 7)) * 16))
+                       : "memory");
+          if (row0 + rr < p.m && col < p.n) {
+            T* dst = static_cast<T*>(p.y) + (row0 + rr) * p.ldy + col;
+            if (vec && col + 16 / ES <= p.n) {
+              *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+              const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+              for (int k = 0; k < 16 / ES; ++k)
+                if (col + k < p.n) dst[k] = e[k];
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
+  if (warp == 8) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        const int ra = mt * 256 + (int)rank * 128, rb = nt * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < nkb; ++kb, ++it) {
+          const int s = it % ST;
+          ok = mbar_wait_cluster(empty(s), ((it / ST) & 1) ^ 1, abort_flag, p.status);
+          if (!ok) break;
+          const uint32_t bar = map_to_rank(full(s), 0);
+          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * L::kStage);
+          const uint32_t dst = base + s * L::kStage;
+          tma_load_2d_pair(dst, &tm_a, kb * kQBlock, ra, bar);
+          tma_load_2d_pair(dst + L::kA, &tm_b, kb * kQBlock, rb, bar);
+        }
+      }
+      // every copy has landed before the CTA may exit: the MMA of its stage has
+      // run (only the leader sees the arrivals themselves)
+      volatile int no_abort = 0;
+      for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i)
+        mbar_wait_cluster(empty(i % ST), (i / ST) & 1, &no_abort, p.status);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    constexpr uint32_t idesc = make_idesc(0, 256, BN);
+    if (lane == 0 && rank == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+        for (int kb = 0; kb < nkb; ++kb, ++it) {
+          const int s = it % ST, b = it & 1;
+          ok = mbar_wait_cluster(acc_empty(b), ((it >> 1) & 1) ^ 1, abort_flag, p.status) &&
+               mbar_wait_cluster(full(s), (it / ST) & 1, abort_flag, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = smem_desc_sw128(base + s * L::kStage);
+          const uint64_t db = smem_desc_sw128(base + s * L::kStage + L::kA);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_e4m3<2>(tmem + b * BN, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), idesc, kk ? 1u : 0u);
+          tc_commit_pair(empty(s));
+          tc_commit_pair(acc_full(b));
+        }
+      }
+      if (it) {  // every MMA has completed before TMEM is freed
+        tc_commit_pair(drain);
+        volatile int no_abort = 0;
+        mbar_wait_cluster(drain, 0, &no_abort, p.status);
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's MMAs read both CTAs' shared memory and write both TMEMs
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, L::kCols);
+  }
+}
+
+// ---------------------------------------------------------------- host
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// Boxes of `box` rows by 128 bytes of a [rows][k] byte matrix, zeros outside.
+bool encode_rows(const uint8_t* q, int rows, int k, int64_t ld, int box, CUtensorMap* map) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t boxes[2] = {128, (cuuint32_t)box}, es[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(q), dims, strides, boxes, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The shared-memory opt-in is a per-device attribute of a kernel.
+template <auto KERNEL>
+int opt_in(int bytes) {
+  constexpr int kMaxDevices = 64;
+  static bool done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return (int)cudaErrorInvalidDevice;
+  if (done[dev]) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done[dev] = true;
+  return (int)e;
+}
+
+template <typename T, int BN>
+int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
+  using L = RowsLayout<BN>;
+  CUtensorMap w, x;
+  if (!encode_rows(a.b, a.n, a.k, a.ldb, 128, &w) || !encode_rows(a.a, a.m, a.k, a.lda, BN, &x))
+    return (int)cudaErrorInvalidValue;
+  int rc = opt_in<matmul_blocks_rows_kernel<T, BN>>(L::kBytes);
+  if (rc) return rc;
+  const int x_tiles = (a.m + BN - 1) / BN;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.n + 127) / 128) * x_tiles * split);
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_rows_kernel<T, BN>, a, w, x, split, x_tiles);
+}
+
+template <typename T, int BN>
+int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st) {
+  using L = PairLayout<BN>;
+  CUtensorMap ma, mb;
+  if (!encode_rows(a.a, a.m, a.k, a.lda, 128, &ma) || !encode_rows(a.b, a.n, a.k, a.ldb, BN / 2, &mb))
+    return (int)cudaErrorInvalidValue;
+  int rc = opt_in<matmul_blocks_pair_kernel<T, BN>>(L::kBytes);
+  if (rc) return rc;
+  const int tiles = ((a.m + 255) / 256) * ((a.n + BN - 1) / BN);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2u * std::min(tiles, num_sms / 2));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN>, a, ma, mb);
+}
+
 }  // namespace
 
 int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st) {
-  (void)num_sms;
+  const bool tma = a.k > 0 && a.lda % 16 == 0 && a.ldb % 16 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b)) & 15) == 0;
   return with_type(a.out_type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    matmul_blocks_simt_kernel<T><<<(unsigned)((a.n + 63) / 64) * ((a.m + 63) / 64), 256, 0, st>>>(a);
-    return (int)cudaGetLastError();
+    if (!tma) {
+      matmul_blocks_simt_kernel<T><<<(unsigned)((a.n + 63) / 64) * ((a.m + 63) / 64), 256, 0, st>>>(a);
+      return (int)cudaGetLastError();
+    }
+    if (a.m > 512) return launch_pair<T, 256>(a, num_sms, st);
+    // split k until about two CTAs per SM run, at least 4 blocks each
+    const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+    const int tiles = ((a.n + 127) / 128) * ((a.m + bn - 1) / bn), kbs = (a.k + kQBlock - 1) / kQBlock;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * num_sms && kbs >= split * 2 * 4) split *= 2;
+    if (bn == 16) return launch_rows<T, 16>(a, split, st);
+    if (bn == 32) return launch_rows<T, 32>(a, split, st);
+    if (bn == 64) return launch_rows<T, 64>(a, split, st);
+    return launch_rows<T, 128>(a, split, st);
   });
 }
 
