@@ -429,7 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(b ? remote_empty1 : remote_empty0);
+              if (lane == 0) mbar_arrive_remote(b ? remote_empty1 : remote_empty0);
             }
             const uint32_t* q = r[g & 1];
 #pragma unroll
@@ -499,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const int ra = mt * 256 + (int)rank * 128, rb = nt * BN + (int)rank * (BN / 2);
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const int s = it % ST;
-          ok = mbar_wait_cluster(empty(s), ((it / ST) & 1) ^ 1, abort_flag, p.status);
+          ok = mbar_wait(empty(s), ((it / ST) & 1) ^ 1, abort_flag, p.status);
           if (!ok) break;
           const uint32_t bar = map_to_rank(full(s), 0);
           if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * L::kStage);
@@ -512,7 +512,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // run (only the leader sees the arrivals themselves)
       volatile int no_abort = 0;
       for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i)
-        mbar_wait_cluster(empty(i % ST), (i / ST) & 1, &no_abort, p.status);
+        mbar_wait(empty(i % ST), (i / ST) & 1, &no_abort, p.status);
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -523,8 +523,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const int s = it % ST, b = it & 1;
-          ok = mbar_wait_cluster(acc_empty(b), ((it >> 1) & 1) ^ 1, abort_flag, p.status) &&
-               mbar_wait_cluster(full(s), (it / ST) & 1, abort_flag, p.status);
+          ok = mbar_wait(acc_empty(b), ((it >> 1) & 1) ^ 1, abort_flag, p.status) &&
+               mbar_wait(full(s), (it / ST) & 1, abort_flag, p.status);
           if (!ok) break;
           tc_fence_after();
           const uint64_t da = smem_desc_sw128(base + s * L::kStage);
@@ -539,7 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (it) {  // every MMA has completed before TMEM is freed
         tc_commit_pair(drain);
         volatile int no_abort = 0;
-        mbar_wait_cluster(drain, 0, &no_abort, p.status);
+        mbar_wait(drain, 0, &no_abort, p.status);
       }
     }
     __syncwarp();

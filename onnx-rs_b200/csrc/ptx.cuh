@@ -408,34 +408,11 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-// mbar_wait for a barrier that other CTAs of the cluster arrive on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                                  int* status) {
-  const auto test = [&]() {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 1000000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-  };
-  if (test()) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!test()) {
-    if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
-      *abort_flag = 1;
-      if (status) atomicCAS(status, 0, ONNXB200_ERR_TIMEOUT);
-      return false;
-    }
-  }
-  return true;
+// Arrival on another CTA's barrier after reads of TMEM, which tcgen05.wait::ld and
+// tcgen05.fence order.  It publishes no generic memory: a release at cluster scope would
+// wait for every load and store of the thread, ~1.5k cycles per 128 k's of a product.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // TMA load into this CTA's shared memory (no multicast) whose completion is signalled on
 // a barrier of either CTA of the pair (a shared::cluster address).
