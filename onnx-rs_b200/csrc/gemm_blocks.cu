@@ -8,12 +8,42 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "blocks.cuh"
 #include "ptx.cuh"
 
 namespace ob2 {
 namespace {
+// Waits without a result: after a wait that gave up (status and abort flag set) the
+// ones behind it return within a millisecond each, and the kernel runs on, over whatever its buffers
+// hold, to its end.  No branch on the outcome, and polling before sleeping: both sit
+// on the round trip between the MMAs and the epilogue that bounds the products.
+__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return;
+  mbar_wait(bar, parity, abort_flag, status);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// Two values rounded to a 16-bit type in one register.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
 // ---------------------------------------------------------------- CUDA cores
 // Operands that TMA cannot read (row strides or pointers off the 16-byte grid):
@@ -281,47 +311,62 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   if (warp < 4) {
     const int j0 = BN * rank / split, j1 = BN * (rank + 1) / split;
     const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
+    uint32_t from[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) from[q] = map_to_rank(mine, q < split ? q : 0);
     for (int j = j0; j < j1; ++j) {
-      float v = 0.f;
-      for (int q = 0; q < split; ++q) v += ld_cluster_f32(map_to_rank(mine + j * 512, q));
-      finish(j, v, bias);
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = ld_cluster_f32(from[q] + j * 512);  // all in flight at once
+#pragma unroll
+      for (int q = 1; q < 8; ++q) v[0] = q < split ? v[0] + v[q] : v[0];
+      finish(j, v[0], bias);
     }
   }
-  cluster_sync();  // no CTA leaves while another reads its partial sums
+  cluster_sync_relaxed();  // no CTA leaves while another reads its partial sums
 }
 
 // ---------------------------------------------------------------- many rows
 // A pair of CTAs computes 256 rows of a by BN rows of b (cta_group::2: each CTA
 // loads its 128 rows of a and half of the rows of b, and holds its 128 rows of
-// the accumulator).  Warps 0-7 of each CTA keep the running totals, thread =
-// row of y, BN / 2 columns each; a row's scale is then one register and the
-// weights' scale the same for all of a warp's columns.  Persistent: pairs walk
-// the tiles, and the next tile's loads and MMAs run during a tile's stores.
+// the accumulator).  The tile's columns are worked on 128 at a time: each half is
+// an accumulator of its own, so its sums are read while the other half's MMAs
+// run, and 128 columns share one scale of b.  Eight warps of each CTA keep the
+// running totals in registers, thread = row of y; a further warp multiplies the
+// scales of a and b and hands them over four blocks at a time.  Persistent: pairs
+// walk the tiles, and a tile's stores (TMA, from shared memory) run under the
+// next tile's loads and MMAs.
+// 8 epilogue warps, then a warpgroup with the TMA, MMA and scale warps.  Launched
+// with 168 registers a thread (384 x 168 = 64512), split as 208 for the totals and
+// 88 for the rest (256 x 208 + 128 x 88 = 64512).
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 384;
+constexpr int kGroupM = 8;  // tile order: columns of 8 tiles, so that pairs running together share operands
+
 template <int BN>
 struct PairLayout {
+  static constexpr int kHalves = BN / 128;
+  static constexpr int kBufs = 4 / kHalves;            // accumulators per half: 512 TMEM columns in all
   static constexpr int kA = 128 * 128, kB = BN / 2 * 128, kStage = kA + kB;
-  static constexpr int kStages = BN == 256 ? 6 : 8;
-  static constexpr int kOut = 8 * 4096;                // per epilogue warp: 32 rows of 128 bytes
+  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr int kRB = 64, kOutBufs = 3;         // staging: rows of 64 bytes, three buffers of 32 rows per warp
+  static constexpr int kOutWarp = kOutBufs * 32 * kRB;
   static constexpr int kOffOut = kStages * kStage;
-  static constexpr int kOffBar = kOffOut + kOut;
-  static constexpr int kBars = 2 * kStages + 5;
+  static constexpr int kOffScale = kOffOut + kPairEpiWarps * kOutWarp;  // two groups: [halves][128] rows of four blocks
+  static constexpr int kScaleGroup = 4 * kHalves * 128;
+  static constexpr int kOffBar = kOffScale + 2 * kScaleGroup * 4;
+  static constexpr int kBars = 2 * kStages + 13;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kBytes = kOffMisc + 16 + 1024;
-  static constexpr int kCols = 2 * BN;                 // two TMEM accumulators
-  static constexpr int kCW = BN / 2;                   // columns per epilogue warp
+  static constexpr int kCW = BN * 4 / kPairEpiWarps;                   // columns per epilogue warp
 };
-// 8 epilogue warps, then a warpgroup with the TMA and the MMA warp.  Launched with
-// 168 registers a thread (3 x 128 x 168 = 64512), split as 208 for the totals and 88
-// for the rest (2 x 128 x 208 + 128 x 88 = 64512).
-constexpr int kPairThreads = 384;
-constexpr int kGroupM = 8;         // tile order: columns of 8 tiles, so that pairs running together share operands
-
 template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     matmul_blocks_pair_kernel(const __grid_constant__ MatmulBlocksArgs p, const __grid_constant__ CUtensorMap tm_a,
-                              const __grid_constant__ CUtensorMap tm_b) {
+                              const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_y,
+                              int tma_out) {
   using L = PairLayout<BN>;
-  constexpr int ST = L::kStages, CW = L::kCW;
+  constexpr int ST = L::kStages, CW = L::kCW, NH = L::kHalves, NB = L::kBufs;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -329,9 +374,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t bar0 = base + L::kOffBar;
   auto full = [&](int s) { return bar0 + 8u * s; };           // leader's: both CTAs' bytes
   auto empty = [&](int s) { return bar0 + 8u * (ST + s); };   // own
-  auto acc_full = [&](int b) { return bar0 + 8u * (2 * ST + b); };
-  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * ST + 2 + b); };  // leader's: 16 warps
-  const uint32_t drain = bar0 + 8u * (2 * ST + 4);
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * ST + b); };       // b = buffer * halves + half
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * ST + 4 + b); };  // leader's: both CTAs' warps
+  auto sc_full = [&](int g) { return bar0 + 8u * (2 * ST + 8 + g); };
+  auto sc_empty = [&](int g) { return bar0 + 8u * (2 * ST + 10 + g); };
+  const uint32_t drain = bar0 + 8u * (2 * ST + 12);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc + 4);
 
@@ -342,18 +389,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 4; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 16);
+      mbar_init(acc_empty(b), 2 * kPairEpiWarps / NH);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(sc_full(g), 32);
+      mbar_init(sc_empty(g), kPairEpiWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
   }
-  if (warp == 9) tmem_alloc_pair(smem_u32(tmem_slot), L::kCols);
-  if (warp == 8 && lane == 0) {
+  if (warp == kPairEpiWarps + 1) tmem_alloc_pair(smem_u32(tmem_slot), 512);
+  if (warp == kPairEpiWarps + 0 && lane == 0) {
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
+    if (tma_out) prefetch_tmap(&tm_y);
   }
   tc_fence_before();
   __syncthreads();
@@ -373,52 +425,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     nt = rem / rows;
   };
 
-  if (warp < 8) {
+  if (warp < kPairEpiWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int sub = warp & 3, half = warp >> 2;
-    const uint32_t lane_addr = tmem + ((uint32_t)(sub * 32) << 16) + half * CW;
-    const uint32_t remote_empty0 = map_to_rank(acc_empty(0), 0), remote_empty1 = map_to_rank(acc_empty(1), 0);
-    const uint32_t out = base + L::kOffOut + warp * 4096;
-    constexpr int ES = sizeof(T), CPR = 128 / ES;  // columns per 128-byte staging row
-    const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.ldy * ES % 16 == 0;
-    uint32_t it = 0;
-    bool ok = true;
-    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
-      int mt, nt;
-      tile_at(t, mt, nt);
-      const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
-      const int col0 = nt * BN + half * CW;
-      const int row = row0 + lane;
-      const float* as = p.as + (int64_t)min(row, p.m - 1) * p.as_row;
-      const float* bs = p.bs + (int64_t)(min(col0, p.n - 1) / kQBlock) * p.bs_row;
+    constexpr int GPH = kPairEpiWarps / 4 / NH;  // groups of four warps per half
+    const int sub = warp & 3, half = (warp >> 2) / GPH, within = (warp >> 2) % GPH * CW;
+    const uint32_t lane_addr = tmem + ((uint32_t)(sub * 32) << 16) + half * 128 + within;
+    const uint32_t remote_empty = map_to_rank(acc_empty(half), 0);
+    const uint32_t sc = base + L::kOffScale + (half * 128 + sub * 32 + lane) * 16;
+    uint32_t it = 0, group = 0;
+    for (int t = blockIdx.x / 2; t < tiles; t += pairs) {
       uint64_t acc[CW / 2];
 #pragma unroll
       for (int j = 0; j < CW / 2; ++j) acc[j] = 0;
-      float na[4], nb[4];  // the next four blocks' scales
-      auto load_scales = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = min(kb + i, nkb - 1);
-          na[i] = as[k * p.as_block];
-          nb[i] = bs[k * p.bs_block];
-        }
-      };
-      load_scales(0);
-      for (int kb = 0; kb < nkb && ok; kb += 4) {
-        float s[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = na[i] * nb[i];
-        if (kb + 4 < nkb) load_scales(kb + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kb + i >= nkb) break;
-          const int b = it & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), (it >> 1) & 1, abort_flag, p.status));
-          if (!ok) break;
+      for (int left = nkb; left > 0; left -= 4, ++group) {
+        const uint32_t g1 = group & 1;
+        bar_wait(sc_full(g1), (group >> 1) & 1, abort_flag, p.status);
+#pragma unroll 1
+        for (int i = 0; i < min(4, left); ++i) {
+          float s;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s) : "r"(sc + g1 * (L::kScaleGroup * 4) + i * 4) : "memory");
+          const uint32_t buf = it % NB;
+          bar_wait(acc_full(buf * NH + half), (it / NB) & 1, abort_flag, p.status);
           ++it;
+          __syncwarp();
           tc_fence_after();
-          const uint64_t s2 = pack_f2(s[i], s[i]);
-          const uint32_t src = lane_addr + b * BN;
+          const uint64_t s2 = pack_f2(s, s);
+          const uint32_t src = lane_addr + buf * (NH * 128);
+          // 16 columns are in flight while the 16 before them are added
           uint32_t r[2][16];
           tmem_ld_32x32b_x16(src, r[0]);
 #pragma unroll
@@ -429,74 +462,110 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_remote(b ? remote_empty1 : remote_empty0);
+              if (lane == 0) mbar_arrive_remote(remote_empty + buf * (NH * 8));
             }
             const uint32_t* q = r[g & 1];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              acc[g * 8 + j] = fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2, acc[g * 8 + j]);
+              acc[g * 8 + j] =
+                  fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2, acc[g * 8 + j]);
           }
-        }
-      }
-      if (!ok) break;
-      // Bias, Relu, rounding; then through shared memory (16-byte units XORed
-      // with the row, free of bank conflicts both ways) so that a warp's stores
-      // are whole 128-byte lines of four rows at a time.
-#pragma unroll
-      for (int c = 0; c < CW / CPR; ++c) {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          uint32_t w[4];
-          T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-          for (int q = 0; q < 16 / ES; ++q) {
-            const int j = c * CPR + u * (16 / ES) + q;
-            const float2 f = unpack_f2(acc[j / 2]);
-            float v = j & 1 ? f.y : f.x;
-            if (p.bias && col0 + j < p.n) v += p.bias[col0 + j];
-            if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays NaN
-            e[q] = from_f32<T>(v);
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((u ^ (lane & 7)) * 16)), "r"(w[0]),
-                       "r"(w[1]), "r"(w[2]), "r"(w[3])
-                       : "memory");
         }
         __syncwarp();
-        const int u = lane & 7, col = col0 + c * CPR + u * (16 / ES);
+        if (lane == 0) mbar_arrive(sc_empty(g1));
+      }
+      // Bias, Relu, rounding; then a warp's 32 rows go through its own staging
+      // rows (swizzled as the TMA map wants them, which is also free of bank
+      // conflicts) to TMA stores that clip the tile's edges; where TMA cannot
+      // write (y off the 16-byte grid), element by element.
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
+      const int col0 = nt * BN + half * 128 + within;
+      constexpr int ES = sizeof(T), CPR = L::kRB / ES;  // columns of a staging row
+      const uint32_t stage0 = base + L::kOffOut + warp * L::kOutWarp + lane * 64;
+      const uint32_t swz = (lane >> 1) & 3;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int rr = q * 4 + (lane >> 3);
+      for (int c = 0; c < CW / CPR; ++c) {
+        if (lane == 0) bulk_wait_group_read<L::kOutBufs - 1>();  // the last store from this buffer has read it
+        __syncwarp();
+        const uint32_t mine = stage0 + c % L::kOutBufs * (32 * L::kRB);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          constexpr int PER = 16 / ES;  // columns of a unit
+          float f[PER];
+#pragma unroll
+          for (int q = 0; q < PER; q += 2) {
+            const float2 v = unpack_f2(acc[(c * CPR + u * PER + q) / 2]);
+            f[q] = v.x;
+            f[q + 1] = v.y;
+          }
+          if (p.bias) {
+            const int j0 = col0 + c * CPR + u * PER;
+#pragma unroll
+            for (int q = 0; q < PER; ++q) f[q] += p.bias[min(j0 + q, p.n - 1)];
+          }
+          if (p.relu) {
+#pragma unroll
+            for (int q = 0; q < PER; ++q) f[q] = f[q] < 0.f ? 0.f : f[q];  // NaN stays NaN
+          }
           uint32_t w[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(out + rr * 128 + ((u ^ (rr & 7)) * 16))
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if constexpr (ES == 4)
+              w[q] = __float_as_uint(f[q]);
+            else
+              w[q] = pack_rounded<T>(f[2 * q], f[2 * q + 1]);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((u ^ swz) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                       "r"(w[3])
                        : "memory");
-          if (row0 + rr < p.m && col < p.n) {
-            T* dst = static_cast<T*>(p.y) + (row0 + rr) * p.ldy + col;
-            if (vec && col + 16 / ES <= p.n) {
-              *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
+        }
+        const int colc = col0 + c * CPR;
+        const uint32_t out = mine - lane * 64;
+        if (tma_out) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < p.m && colc < p.n) tma_store_2d(&tm_y, colc, row0, out);
+            bulk_commit_group();
+          }
+        } else {
+          __syncwarp();
+          const int u = lane & 3, col = colc + u * (16 / ES);
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            const int rr = q * 8 + (lane >> 2);
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(out + rr * 64 + ((u ^ ((rr >> 1) & 3)) * 16))
+                         : "memory");
+            if (row0 + rr < p.m) {
+              T* dst = static_cast<T*>(p.y) + (row0 + rr) * p.ldy + col;
               const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
               for (int k = 0; k < 16 / ES; ++k)
                 if (col + k < p.n) dst[k] = e[k];
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
     }
+    if (lane == 0) bulk_wait_group<0>();  // every store is complete before the CTA exits
+    __syncwarp();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
-  if (warp == 8) {
+  if (warp == kPairEpiWarps + 0) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
       for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
         int mt, nt;
         tile_at(t, mt, nt);
-        const int ra = mt * 256 + (int)rank * 128, rb = nt * BN + (int)rank * (BN / 2);
+        const int ra = mt * 256 + (int)rank * 128, rb = nt * BN + (int)rank * 64;
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const int s = it % ST;
           ok = mbar_wait(empty(s), ((it / ST) & 1) ^ 1, abort_flag, p.status);
@@ -505,51 +574,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * L::kStage);
           const uint32_t dst = base + s * L::kStage;
           tma_load_2d_pair(dst, &tm_a, kb * kQBlock, ra, bar);
-          tma_load_2d_pair(dst + L::kA, &tm_b, kb * kQBlock, rb, bar);
+#pragma unroll
+          for (int hf = 0; hf < NH; ++hf)  // this CTA's 64 rows of each half
+            tma_load_2d_pair(dst + L::kA + hf * 8192, &tm_b, kb * kQBlock, rb + hf * 128, bar);
         }
       }
       // every copy has landed before the CTA may exit: the MMA of its stage has
       // run (only the leader sees the arrivals themselves)
       volatile int no_abort = 0;
-      for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i)
-        mbar_wait(empty(i % ST), (i / ST) & 1, &no_abort, p.status);
+      for (uint32_t i = it > ST ? it - ST : 0; i < it; ++i) mbar_wait(empty(i % ST), (i / ST) & 1, &no_abort, p.status);
     }
     __syncwarp();
-  } else if (warp == 9) {
-    constexpr uint32_t idesc = make_idesc(0, 256, BN);
-    if (lane == 0 && rank == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % ST, b = it & 1;
-          ok = mbar_wait(acc_empty(b), ((it >> 1) & 1) ^ 1, abort_flag, p.status) &&
-               mbar_wait(full(s), (it / ST) & 1, abort_flag, p.status);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t da = smem_desc_sw128(base + s * L::kStage);
-          const uint64_t db = smem_desc_sw128(base + s * L::kStage + L::kA);
+  } else if (warp == kPairEpiWarps + 1) {
+    constexpr uint32_t idesc = make_idesc(0, 256, 128);
+    if (rank == 0) {
+      const bool leader = elect_one();
+      int s = 0, buf = 0;
+      uint32_t sp = 0, bp = 1;  // parities: of the stage's use, of the buffer's release
+      const int total = nkb * ((tiles - (int)(blockIdx.x / 2) + pairs - 1) / pairs);
+      for (int it = 0; it < total; ++it) {
+        const uint64_t da = smem_desc_sw128(base + s * L::kStage);
+        const uint64_t db = smem_desc_sw128(base + s * L::kStage + L::kA);
+        bar_wait(full(s), sp, abort_flag, p.status);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_e4m3<2>(tmem + b * BN, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), idesc, kk ? 1u : 0u);
-          tc_commit_pair(empty(s));
-          tc_commit_pair(acc_full(b));
+        for (int hf = 0; hf < NH; ++hf) {
+          bar_wait(acc_empty(buf * NH + hf), bp, abort_flag, p.status);
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_e4m3<2>(tmem + (buf * NH + hf) * 128, da + (uint64_t)(kk * 2), db + (uint64_t)(hf * 512 + kk * 2),
+                             idesc, kk ? 1u : 0u);
+            if (hf == NH - 1) tc_commit_pair(empty(s));
+            tc_commit_pair(acc_full(buf * NH + hf));
+          }
+        }
+        if (++s == ST) {
+          s = 0;
+          sp ^= 1;
+        }
+        if (++buf == NB) {
+          buf = 0;
+          bp ^= 1;
         }
       }
-      if (it) {  // every MMA has completed before TMEM is freed
+      // every MMA has completed before TMEM is freed
+      if (leader) {
         tc_commit_pair(drain);
         volatile int no_abort = 0;
         mbar_wait(drain, 0, &no_abort, p.status);
       }
     }
     __syncwarp();
+  } else if (warp == kPairEpiWarps + 2) {
+    // sa * sb of this CTA's 128 rows and each half's block of b, four blocks of k
+    // ahead: loaded before the buffer is waited for
+    uint32_t group = 0;
+    bool ok = true;
+    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row = mt * 256 + (int)rank * 128 + lane;
+      for (int kb = 0; kb < nkb; kb += 4, ++group) {
+        float va[4][4], vb[4][NH];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = min(kb + i, nkb - 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) va[i][j] = p.as[(int64_t)min(row + j * 32, p.m - 1) * p.as_row + k * p.as_block];
+#pragma unroll
+          for (int hf = 0; hf < NH; ++hf)
+            vb[i][hf] = p.bs[(int64_t)(min(nt * BN + hf * 128, p.n - 1) / kQBlock) * p.bs_row + k * p.bs_block];
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(sc_empty(group & 1), ((group >> 1) & 1) ^ 1, abort_flag, p.status));
+        if (!ok) break;
+        float4* dst = reinterpret_cast<float4*>(gbase + L::kOffScale) + (group & 1) * (L::kScaleGroup / 4) + lane;
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dst[hf * 128 + j * 32] = make_float4(va[0][j] * vb[0][hf], va[1][j] * vb[1][hf], va[2][j] * vb[2][hf], va[3][j] * vb[3][hf]);
+        mbar_arrive(sc_full(group & 1));  // every lane: its own stores
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // the pair's MMAs read both CTAs' shared memory and write both TMEMs
-  if (warp == 9) {
+  if (warp == kPairEpiWarps + 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, L::kCols);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -618,12 +732,25 @@ int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
   return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_rows_kernel<T, BN>, a, w, x, split, x_tiles);
 }
 
+// Boxes of 32 rows by `box_bytes` of y, for the stores; false where TMA cannot write.
+template <typename T>
+bool encode_out(const MatmulBlocksArgs& a, int box_bytes, CUtensorMap* map) {
+  EncodeFn fn = encode_fn();
+  if (!fn || (reinterpret_cast<uintptr_t>(a.y) & 15) || a.ldy * sizeof(T) % 16) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)a.n, (cuuint64_t)a.m}, strides[1] = {(cuuint64_t)a.ldy * sizeof(T)};
+  const cuuint32_t boxes[2] = {(cuuint32_t)(box_bytes / sizeof(T)), 32}, es[2] = {1, 1};
+  return fn(map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a.y, dims, strides,
+            boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int BN>
 int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st) {
   using L = PairLayout<BN>;
-  CUtensorMap ma, mb;
-  if (!encode_rows(a.a, a.m, a.k, a.lda, 128, &ma) || !encode_rows(a.b, a.n, a.k, a.ldb, BN / 2, &mb))
+  CUtensorMap ma, mb, my{};
+  if (!encode_rows(a.a, a.m, a.k, a.lda, 128, &ma) || !encode_rows(a.b, a.n, a.k, a.ldb, 64, &mb))
     return (int)cudaErrorInvalidValue;
+  const int tma_out = encode_out<T>(a, L::kRB, &my);
   int rc = opt_in<matmul_blocks_pair_kernel<T, BN>>(L::kBytes);
   if (rc) return rc;
   const int tiles = ((a.m + 255) / 256) * ((a.n + BN - 1) / BN);
@@ -637,7 +764,7 @@ int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN>, a, ma, mb);
+  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN>, a, ma, mb, my, tma_out);
 }
 
 }  // namespace
@@ -651,16 +778,21 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       matmul_blocks_simt_kernel<T><<<(unsigned)((a.n + 63) / 64) * ((a.m + 63) / 64), 256, 0, st>>>(a);
       return (int)cudaGetLastError();
     }
-    if (a.m > 512) return launch_pair<T, 256>(a, num_sms, st);
-    // split k until about two CTAs per SM run, at least 4 blocks each
-    const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
-    const int tiles = ((a.n + 127) / 128) * ((a.m + bn - 1) / bn), kbs = (a.k + kQBlock - 1) / kQBlock;
+    const int kbs = (a.k + kQBlock - 1) / kQBlock;
+    if (a.m > 32) {
+      // Tiles of 256 x 256 or 256 x 128 on num_sms / 2 pairs: a wave of the narrow
+      // ones takes ~0.6 of a wave of the wide ones (8.5 and 16 us at k = 4096; 200 x
+      // 8192: 15.3 and 20.4 us, 512 x 8192: 23.4 and 21.4 us, 4096 x 4096: 70.6 and 67.2 us).
+      const int64_t tm = (a.m + 255) / 256, pairs = num_sms / 2;
+      const int64_t wide = (tm * ((a.n + 255) / 256) + pairs - 1) / pairs, narrow = (tm * ((a.n + 127) / 128) + pairs - 1) / pairs;
+      return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
+    }
+    // split k until about one CTA per SM runs, at least 4 blocks each (1 x 4096 x
+    // 4096: 15.3, 11.6, 9.2 and 17.0 us with 1, 2, 4 and 8 CTAs per tile)
+    const int tiles = (a.n + 127) / 128;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= 2 * num_sms && kbs >= split * 2 * 4) split *= 2;
-    if (bn == 16) return launch_rows<T, 16>(a, split, st);
-    if (bn == 32) return launch_rows<T, 32>(a, split, st);
-    if (bn == 64) return launch_rows<T, 64>(a, split, st);
-    return launch_rows<T, 128>(a, split, st);
+    while (split < 8 && tiles * split * 2 <= num_sms && kbs >= split * 2 * 4) split *= 2;
+    return a.m <= 16 ? launch_rows<T, 16>(a, split, st) : launch_rows<T, 32>(a, split, st);
   });
 }
 
