@@ -52,6 +52,28 @@ __device__ __forceinline__ float from_e4m3(uint8_t v) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
 }
 
+// Programmatic dependent launch: the kernel's blocks may start while the previous
+// kernel on the stream ends, and wait here before they touch global memory; the
+// next kernel's may start once all of this one's have.
+__device__ __forceinline__ void pdl_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+int launch_pdl(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // Calls f with a null pointer of the element type `t` (F32, F16 or BF16).
 template <typename F>
 auto with_type(int t, F f) {

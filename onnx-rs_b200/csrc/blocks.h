@@ -29,7 +29,7 @@ struct RmsNormArgs {
   float eps;
 };
 // Return a cudaError_t.
-int rmsnorm_launch(const RmsNormArgs& a, cudaStream_t stream);
+int rmsnorm_launch(const RmsNormArgs& a, int num_sms, cudaStream_t stream);
 
 struct QuantizeArgs {
   const void* x;

@@ -102,7 +102,7 @@ int onnxb200_rmsnorm(onnxb200_handle* h, const onnxb200_rmsnorm_desc* d, const v
     return fail(h, ONNXB200_ERR_VALIDATION, "RMSNormalization: pointer not aligned to its type");
   if (!h) return ONNXB200_ERR_INVALID_ARGUMENT;
   DeviceGuard g(h->device);
-  const int rc = rmsnorm_launch(a, h->stream);
+  const int rc = rmsnorm_launch(a, h->num_sms, h->stream);
   h->launches++;
   return rc ? cuda_fail(h, rc, "RMSNormalization") : ONNXB200_OK;
 }

@@ -52,6 +52,7 @@ __device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
 template <typename T>
 __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlocksArgs p) {
   __shared__ float sa[32][65], sb[32][65];
+  pdl_begin();
   const int tiles_n = (p.n + 63) / 64;
   const int m0 = blockIdx.x / tiles_n * 64, n0 = blockIdx.x % tiles_n * 64;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -168,8 +169,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  pdl_begin();
 
   const int rank = blockIdx.x % split;
   const int tile = blockIdx.x / split;
@@ -412,8 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();  // both CTAs' barriers are initialised
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  pdl_begin();
 
   const int tm = (p.m + 255) / 256, tn = (p.n + BN - 1) / BN;
   const int tiles = tm * tn, pairs = gridDim.x / 2;
@@ -775,8 +774,7 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
   return with_type(a.out_type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (!tma) {
-      matmul_blocks_simt_kernel<T><<<(unsigned)((a.n + 63) / 64) * ((a.m + 63) / 64), 256, 0, st>>>(a);
-      return (int)cudaGetLastError();
+      return launch_pdl(matmul_blocks_simt_kernel<T>, (unsigned)((a.n + 63) / 64) * ((a.m + 63) / 64), 256, 0, st, a);
     }
     const int kbs = (a.k + kQBlock - 1) / kQBlock;
     if (a.m > 32) {
