@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "blocks.h"
 
 namespace ob2 {
@@ -26,6 +28,23 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// max_nan(m, |v|)
+__device__ __forceinline__ float max_abs_nan(float m, float v) {
+  float r;
+  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(m), "f"(v));
+  return r;
+}
+
+// Two values rounded to a 16-bit type in one register.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 

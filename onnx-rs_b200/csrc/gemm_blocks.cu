@@ -8,7 +8,6 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "blocks.cuh"
 #include "ptx.cuh"
@@ -32,17 +31,6 @@ __device__ __forceinline__ bool elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(p));
   return p != 0;
-}
-
-// Two values rounded to a 16-bit type in one register.
-template <typename T>
-__device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same_v<T, __half>)
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
 }
 
 // ---------------------------------------------------------------- CUDA cores

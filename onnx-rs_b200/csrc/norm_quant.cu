@@ -22,24 +22,115 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 // two 16-byte accesses, 16-bit types: one).
 template <typename T>
 struct Vec8 {
-  uint4 v[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
+  uint32_t v[2 * sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, bool in_range) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 u = in_range ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+      v[i * 4] = u.x;
+      v[i * 4 + 1] = u.y;
+      v[i * 4 + 2] = u.z;
+      v[i * 4 + 3] = u.w;
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (std::is_same_v<T, float>)
+        f[i] = __uint_as_float(v[i]);
+      else if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        f[i] = __uint_as_float(i & 1 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
+      else
+        f[i] = __half2float(__ushort_as_half((unsigned short)(v[i / 2] >> (i & 1 ? 16 : 0))));
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&f)[8]) {
+    if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = pack_rounded<T>(f[2 * i], f[2 * i + 1]);
+    }
   }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(v[i * 4], v[i * 4 + 1], v[i * 4 + 2], v[i * 4 + 3]);
   }
-  __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(v)[i]); }
-  __device__ __forceinline__ void set(int i, float f) { reinterpret_cast<T*>(v)[i] = from_f32<T>(f); }
+  // Largest magnitude; 16-bit types two at a time, in their own type (it is exact).
+  __device__ __forceinline__ float amax() const {
+    if constexpr (std::is_same_v<T, float>) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max_abs_nan(m, __uint_as_float(v[i]));
+      return m;
+    } else {
+      uint32_t m = v[0] & 0x7fff7fffu;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        if constexpr (std::is_same_v<T, __half>)
+          asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(v[i] & 0x7fff7fffu));
+        else
+          asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(v[i] & 0x7fff7fffu));
+      }
+      const unsigned short lo = (unsigned short)m, hi = (unsigned short)(m >> 16);
+      if constexpr (std::is_same_v<T, __half>)
+        return max_nan(__half2float(__ushort_as_half(lo)), __half2float(__ushort_as_half(hi)));
+      else
+        return max_nan(__uint_as_float((uint32_t)lo << 16), __uint_as_float((uint32_t)hi << 16));
+    }
+  }
 };
 
-// Largest magnitude over the 16 lanes (of 8 elements each) that share a block of 128.
-__device__ __forceinline__ float lanes16_max_nan(float v) {
+// Eight values times inv, in e4m3.
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], float inv) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(to_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                                            to_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+
+// The scales of N vectors (1, 2 or 4) per lane, each vector's block being spread
+// over the 16 lanes of a half warp: `amax` holds a lane's largest magnitudes, inv[c]
+// receives the factor of vector c's block.  The maxima are exchanged so that each
+// lane ends with one block's, and the two divisions of a block are done by one lane
+// in four or so instead of by all 16: they were a quarter of all instructions of
+// kernels whose instructions, not bytes, set the time.  The block that a lane ended
+// with is returned, and its scale.
+template <int N>
+__device__ __forceinline__ int half_warp_scales(const float (&amax)[N], float (&inv)[N], float& scale) {
+  const int lane = threadIdx.x & 31;
+  float m;
+  int mine;
+  if constexpr (N == 4) {
+    const bool up = lane & 8, up2 = lane & 4;
+    float a = up ? amax[2] : amax[0], b = up ? amax[3] : amax[1];
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, up ? amax[0] : amax[2], 8));
+    b = max_nan(b, __shfl_xor_sync(0xffffffffu, up ? amax[1] : amax[3], 8));
+    m = max_nan(up2 ? b : a, __shfl_xor_sync(0xffffffffu, up2 ? a : b, 4));
+    mine = (lane >> 2) & 3;
+  } else if constexpr (N == 2) {
+    const bool up = lane & 8;
+    m = max_nan(up ? amax[1] : amax[0], __shfl_xor_sync(0xffffffffu, up ? amax[0] : amax[1], 8));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    mine = (lane >> 3) & 1;
+  } else {
+    m = max_nan(amax[0], __shfl_xor_sync(0xffffffffu, amax[0], 8));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    mine = 0;
+  }
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  float f;
+  block_scale(m, scale, f);
 #pragma unroll
-  for (int o = 8; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  for (int c = 0; c < N; ++c)
+    inv[c] = N == 1 ? f : __shfl_sync(0xffffffffu, f, (lane & 16) | c * (16 / N));
+  return mine;
+}
+// Whether this lane writes the scale it ended with.
+template <int N>
+__device__ __forceinline__ bool writes_scale() {
+  return (threadIdx.x & (16 / N - 1)) == 0;
 }
 
 // Rows whose every vector is aligned: one row per block, CH vectors of eight
@@ -56,32 +147,35 @@ __global__ void __launch_bounds__(CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 
   pdl_begin();
   const int64_t r = blockIdx.x;
   const int n8 = p.cols / 8, nt = blockDim.x;
+  // vector c of this thread; threads past the row's end work on zeros
+  auto at = [&](int c) { return c * nt + (int)threadIdx.x; };
   const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-  Vec8<T> v[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-    if (c * nt + threadIdx.x < n8) v[c].load(x + (c * nt + threadIdx.x) * 8);
   float h[CH][8];
-  if (p.res) {
-    const T* res = static_cast<const T*>(p.res) + r * p.ldr;
-    Vec8<T> vr[CH];
+  {
+    Vec8<T> v[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-      if (c * nt + threadIdx.x < n8) vr[c].load(res + (c * nt + threadIdx.x) * 8);
+    for (int c = 0; c < CH; ++c) v[c].load(x + at(c) * 8, at(c) < n8);
+    if (p.res) {
+      const T* res = static_cast<const T*>(p.res) + r * p.ldr;
+      Vec8<T> vr[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c) vr[c].load(res + at(c) * 8, at(c) < n8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[c][j] = c * nt + threadIdx.x < n8 ? v[c].get(j) + vr[c].get(j) : 0.f;
-  } else {
+      for (int c = 0; c < CH; ++c) {
+        float f[8];
+        v[c].unpack(h[c]);
+        vr[c].unpack(f);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+        for (int j = 0; j < 8; ++j) h[c][j] += f[j];
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[c][j] = c * nt + threadIdx.x < n8 ? v[c].get(j) : 0.f;
+      for (int c = 0; c < CH; ++c) v[c].unpack(h[c]);
+    }
   }
   Vec8<W> vw[CH];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-    if (c * nt + threadIdx.x < n8) vw[c].load(static_cast<const W*>(p.weight) + (c * nt + threadIdx.x) * 8);
+  for (int c = 0; c < CH; ++c) vw[c].load(static_cast<const W*>(p.weight) + at(c) * 8, at(c) < n8);
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
@@ -94,41 +188,45 @@ __global__ void __launch_bounds__(CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       Vec8<T> o;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o.set(j, h[c][j]);
-      if (c * nt + threadIdx.x < n8) o.store(sum + (c * nt + threadIdx.x) * 8);
+      o.pack(h[c]);
+      if (at(c) < n8) o.store(sum + at(c) * 8);
     }
   }
   __syncthreads();
   ss = (threadIdx.x & 31) < nt / 32 ? part[threadIdx.x & 31] : 0.f;
   ss = warp_sum(ss);
   const float rstd = 1.f / sqrtf(ss / (float)p.cols + p.eps);
+  float amax[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int i = c * nt + threadIdx.x;
-    float amax = 0.f;
+    float f[8];
+    vw[c].unpack(f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      h[c][j] = i < n8 ? h[c][j] * rstd * vw[c].get(j) : 0.f;
-      amax = max_nan(amax, fabsf(h[c][j]));
-    }
-    if (p.out_type != kE4M3) {
-      Vec8<T> o;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o.set(j, h[c][j]);
-      if (i < n8) o.store(static_cast<T*>(p.y) + r * p.ldy + i * 8);
-    } else {
-      float scale, inv;
-      block_scale(lanes16_max_nan(amax), scale, inv);
-      if (i < n8) {
-        const float* f = h[c];
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.y) + r * p.ldy + i * 8) =
-            make_uint2(to_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                       to_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-        if ((threadIdx.x & 15) == 0) p.y_scale[r * p.ys_row + (i / 16) * p.ys_block] = scale;
-      }
-    }
+    for (int j = 0; j < 8; ++j) h[c][j] = h[c][j] * rstd * f[j];
   }
+  if (p.out_type != kE4M3) {
+    T* y = static_cast<T*>(p.y) + r * p.ldy;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      Vec8<T> o;
+      o.pack(h[c]);
+      if (at(c) < n8) o.store(y + at(c) * 8);
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    amax[c] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax[c] = max_abs_nan(amax[c], h[c][j]);
+  }
+  float inv[CH], scale;
+  const int mine = at(half_warp_scales<CH>(amax, inv, scale)) / 16;
+  if (writes_scale<CH>() && mine * 16 < n8) p.y_scale[r * p.ys_row + mine * p.ys_block] = scale;
+  uint8_t* q = static_cast<uint8_t*>(p.y) + r * p.ldy;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    if (at(c) < n8) store_e4m3(q + at(c) * 8, h[c], inv[c]);
 }
 
 // Any alignment and width: one row per block, the row's fp32 sum x + residual held
@@ -198,7 +296,6 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_row_kernel(const RmsNormA
 // block_rows = 1, aligned rows: a warp takes UNROLL x 256 columns of a row, eight
 // per lane and vector (2 or 4 KB a warp), all loads in flight before the first is used; 16 lanes
 // share a block's scale.  Bound by HBM: 8192 x 4096 fp32 (169 MB) in %QROW%.
-template <typename T>
 constexpr int kQuantUnroll = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_row_vec_kernel(const QuantizeArgs p, unsigned segments, unsigned units) {
@@ -206,28 +303,22 @@ __global__ void __launch_bounds__(256) quantize_row_vec_kernel(const QuantizeArg
   const unsigned u = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (u >= units) return;
   const int64_t r = u / segments;
-  const int n8 = (int)(p.cols / 8), i0 = (int)(u % segments) * (kQuantUnroll<T> * 32) + (threadIdx.x & 31);
+  const int n8 = (int)(p.cols / 8), i0 = (int)(u % segments) * (kQuantUnroll * 32) + (threadIdx.x & 31);
   const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-  Vec8<T> v[kQuantUnroll<T>];
+  Vec8<T> v[kQuantUnroll];
 #pragma unroll
-  for (int c = 0; c < kQuantUnroll<T>; ++c)
-    if (i0 + c * 32 < n8) v[c].load(x + (int64_t)(i0 + c * 32) * 8);
+  for (int c = 0; c < kQuantUnroll; ++c) v[c].load(x + (int64_t)(i0 + c * 32) * 8, i0 + c * 32 < n8);
+  float amax[kQuantUnroll], inv[kQuantUnroll], scale;
 #pragma unroll
-  for (int c = 0; c < kQuantUnroll<T>; ++c) {
-    const int i = i0 + c * 32;
-    float amax = 0.f;
-    if (i < n8) {
+  for (int c = 0; c < kQuantUnroll; ++c) amax[c] = v[c].amax();
+  const int mine = (i0 + half_warp_scales<kQuantUnroll>(amax, inv, scale) * 32) / 16;
+  if (writes_scale<kQuantUnroll>() && mine * 16 < n8) p.scale[r * p.s_row + mine * p.s_block] = scale;
+  uint8_t* q = p.q + r * p.ldq;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[c].get(j)));
-    }
-    float scale, inv;
-    block_scale(lanes16_max_nan(amax), scale, inv);
-    if (i < n8) {
-      *reinterpret_cast<uint2*>(p.q + r * p.ldq + (int64_t)i * 8) =
-          make_uint2(to_e4m3x4(v[c].get(0) * inv, v[c].get(1) * inv, v[c].get(2) * inv, v[c].get(3) * inv),
-                     to_e4m3x4(v[c].get(4) * inv, v[c].get(5) * inv, v[c].get(6) * inv, v[c].get(7) * inv));
-      if ((threadIdx.x & 15) == 0) p.scale[r * p.s_row + (i / 16) * p.s_block] = scale;
-    }
+  for (int c = 0; c < kQuantUnroll; ++c) {
+    float f[8];
+    v[c].unpack(f);
+    if (i0 + c * 32 < n8) store_e4m3(q + (int64_t)(i0 + c * 32) * 8, f, inv[c]);
   }
 }
 
@@ -278,64 +369,88 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tile_vec
   const int64_t c = b * kQBlock + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
   const T* x = static_cast<const T*>(p.x);
   Vec8<T> v[8];
+  auto in_range = [&](int i) { return c < p.cols && r0 + i * 16 < p.rows; };
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c < p.cols && r0 + i * 16 < p.rows) v[i].load(x + (r0 + i * 16) * p.ldx + c);
+  for (int i = 0; i < 8; ++i) v[i].load(x + (r0 + i * 16) * p.ldx + c, in_range(i));
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c < p.cols && r0 + i * 16 < p.rows) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i].get(j)));
-    }
+  for (int i = 0; i < 8; ++i) amax = max_nan(amax, v[i].amax());
   float scale, inv;
   block_scale(block_max_nan(amax), scale, inv);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c < p.cols && r0 + i * 16 < p.rows)
-      *reinterpret_cast<uint2*>(p.q + (r0 + i * 16) * p.ldq + c) =
-          make_uint2(to_e4m3x4(v[i].get(0) * inv, v[i].get(1) * inv, v[i].get(2) * inv, v[i].get(3) * inv),
-                     to_e4m3x4(v[i].get(4) * inv, v[i].get(5) * inv, v[i].get(6) * inv, v[i].get(7) * inv));
+  for (int i = 0; i < 8; ++i) {
+    float f[8];
+    v[i].unpack(f);
+    if (in_range(i)) store_e4m3(p.q + (r0 + i * 16) * p.ldq + c, f, inv);
+  }
   if (threadIdx.x == 0) p.scale[rb * p.s_row + b * p.s_block] = scale;
 }
 
 // block_rows = 128, any alignment: V elements per access (2 where rows start on
-// multiples of two elements).  The block is read twice, the second time from L2:
-// keeping it in registers left too few of them for more than one block per SM.
+// multiples of two elements), eight rows of loads in flight; the block is read a
+// second time, from L2 (in registers it left room for one block per SM, or was
+// slower by its guards).  5000 x 2050 bf16 (31 MB): %QTILE%.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) quantize_tile_kernel(const QuantizeArgs p, unsigned cb) {
   pdl_begin();
   struct alignas(sizeof(T) * V) Elems { T e[V]; };
   struct alignas(V) Bytes { uint8_t e[V]; };
-  constexpr int kAcross = 128 / V, kDown = 256 / kAcross;
+  constexpr int kAcross = 128 / V, kDown = 256 / kAcross, kBatch = 8;
   const int64_t rb = blockIdx.x / cb, b = blockIdx.x % cb;
   const int64_t c = b * kQBlock + threadIdx.x % kAcross * V, r0 = rb * 128 + threadIdx.x / kAcross;
-  const T* x = static_cast<const T*>(p.x) + r0 * p.ldx + c;
-  const int rows = c < p.cols ? (int)min((int64_t)128, p.rows - rb * 128) - (int)(threadIdx.x / kAcross) : 0;
-  float amax = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < rows; i += kDown) {
-    const Elems v = *reinterpret_cast<const Elems*>(x + i * p.ldx);
+  const char* x = reinterpret_cast<const char*>(static_cast<const T*>(p.x) + r0 * p.ldx + c);
+  const int64_t step = kDown * p.ldx * (int64_t)sizeof(T), qstep = kDown * p.ldq;
+  uint8_t* q = p.q + r0 * p.ldq + c;
+  // rows of this thread: r0 + i * kDown for i < mine
+  const int left = c < p.cols ? (int)min((int64_t)128, p.rows - rb * 128) - (int)(threadIdx.x / kAcross) : 0;
+  const int mine = left > 0 ? (left + kDown - 1) / kDown : 0;
+  auto amax_of = [](const Elems& v) {
+    float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) amax = max_nan(amax, fabsf(to_f32(v.e[j])));
-  }
+    for (int j = 0; j < V; ++j) m = max_abs_nan(m, to_f32(v.e[j]));
+    return m;
+  };
+  auto put = [&](uint8_t* to, const Elems& v, float inv) {
+    Bytes w;
+    if constexpr (V == 2) {
+      uint16_t two;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(to_f32(v.e[1]) * inv), "f"(to_f32(v.e[0]) * inv));
+      *reinterpret_cast<uint16_t*>(to) = two;
+    } else {
+      w.e[0] = to_e4m3(to_f32(v.e[0]) * inv);
+      *reinterpret_cast<Bytes*>(to) = w;
+    }
+  };
+  // f(pointer, row index) over this thread's rows, kBatch at a time
+  auto walk = [&](auto batch, auto single) {
+    const char* at = x;
+    int i = 0;
+    for (; i + kBatch <= mine; i += kBatch) {
+      Elems v[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k, at += step) v[k] = *reinterpret_cast<const Elems*>(at);
+      batch(v);
+    }
+    for (; i < mine; ++i, at += step) single(*reinterpret_cast<const Elems*>(at));
+  };
+  float amax = 0.f;
+  walk(
+      [&](const Elems (&v)[kBatch]) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) amax = max_nan(amax, amax_of(v[k]));
+      },
+      [&](const Elems& v) { amax = max_nan(amax, amax_of(v)); });
   float scale, inv;
   block_scale(block_max_nan(amax), scale, inv);
-  uint8_t* q = p.q + r0 * p.ldq + c;
-  for (int i0 = 0; i0 < rows; i0 += 8 * kDown) {
-    Elems v[8];
+  walk(
+      [&](const Elems (&v)[kBatch]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i0 + k * kDown < rows) v[k] = *reinterpret_cast<const Elems*>(x + (i0 + k * kDown) * p.ldx);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (i0 + k * kDown >= rows) break;
-      Bytes w;
-#pragma unroll
-      for (int j = 0; j < V; ++j) w.e[j] = to_e4m3(to_f32(v[k].e[j]) * inv);
-      *reinterpret_cast<Bytes*>(q + (i0 + k * kDown) * p.ldq) = w;
-    }
-  }
+        for (int k = 0; k < kBatch; ++k, q += qstep) put(q, v[k], inv);
+      },
+      [&](const Elems& v) {
+        put(q, v, inv);
+        q += qstep;
+      });
   if (threadIdx.x == 0) p.scale[rb * p.s_row + b * p.s_block] = scale;
 }
 
@@ -384,7 +499,7 @@ int quantize_launch(const QuantizeArgs& a, cudaStream_t st) {
     const bool vec = a.cols % 8 == 0 && on_grid(a.x, a.ldx, sizeof(T), 16) && on_grid(a.q, a.ldq, 1, 8);
     if (a.block_rows == 1) {
       if (vec) {
-        const unsigned per = kQuantUnroll<T> * 256, segments = (unsigned)((a.cols + per - 1) / per);
+        const unsigned per = kQuantUnroll * 256, segments = (unsigned)((a.cols + per - 1) / per);
         const unsigned units = (unsigned)a.rows * segments;
         return launch_pdl(quantize_row_vec_kernel<T>, (units + 7) / 8, 256, 0, st, a, segments, units);
       }

@@ -551,20 +551,35 @@ def _row_stride(t, what):
     return ld
 
 
-def _stored_rows(lead, cols, dev):
-    """Uninitialised e4m3 tensor [*lead, cols] whose rows start on 16-byte boundaries (what the
-    tensor-core product reads), with its row stride."""
-    ld = (cols + 15) // 16 * 16
-    if ld == cols:
-        return torch.empty((*lead, cols), dtype=_E4M3, device=dev), ld
-    return torch.empty((*lead, ld), dtype=_E4M3, device=dev)[..., :cols], ld
+def _stored_stride(cols):
+    """Row stride of e4m3 rows that start on 16-byte boundaries (what the tensor-core product reads)."""
+    return (cols + 15) // 16 * 16
 
 
-def _stored_scales(lead, rows, blocks, dev):
-    """Uninitialised scales [*lead, blocks]; those of one block of columns lie side by side, as the
-    product reads them."""
-    s = torch.empty((blocks, rows), dtype=torch.float32, device=dev).t()
-    return s if len(lead) == 1 else s.unflatten(0, lead) if lead else s[0]
+def _dense(shape, dtype):
+    """(shape, strides, dtype) of a new contiguous tensor."""
+    strides, step = [], 1
+    for n in reversed(shape):
+        strides.append(step)
+        step *= max(1, n)
+    return tuple(shape), tuple(reversed(strides)), dtype
+
+
+def _stored_rows(lead, cols):
+    """(shape, strides, dtype) of new e4m3 rows [*lead, cols], _stored_stride(cols) apart."""
+    _, strides, _ = _dense((*lead, _stored_stride(cols)), _E4M3)
+    return (*lead, cols), strides, _E4M3
+
+
+def _stored_scales(lead, rows, blocks):
+    """(shape, strides, dtype) of new scales [*lead, blocks]; those of one block of columns lie side by
+    side, as the product reads them."""
+    _, strides, _ = _dense(lead, torch.float32)
+    return (*lead, blocks), (*strides, max(1, rows)), torch.float32
+
+
+def _new(spec, dev):
+    return torch.empty_strided(spec[0], spec[1], dtype=spec[2], device=dev)
 
 
 def _scale_strides(s, rows, blocks, what):
@@ -584,15 +599,16 @@ def _scale_strides(s, rows, blocks, what):
 
 def _launch(h, what, entry, desc, *args):
     """Calls a C entry in order with torch's current stream, whatever stream the handle runs on."""
-    cur = torch.cuda.current_stream(h.device)
+    cur = torch._C._cuda_getCurrentRawStream(h.device)
     run = h.stream_ptr
-    side = None
     # the handle's own stream is a blocking one: ordered with the legacy default stream by itself
-    if cur.cuda_stream != run and not (cur.cuda_stream == 0 and run == h.own_stream_ptr):
+    if cur == run or (cur == 0 and run == h.own_stream_ptr):
+        rc = entry(h.ptr, desc, *args)
+    else:
+        cur = torch.cuda.current_stream(h.device)
         side = torch.cuda.ExternalStream(run, device=h.device)
         side.wait_stream(cur)
-    rc = entry(h.ptr, ctypes.byref(desc), *args)
-    if side is not None:
+        rc = entry(h.ptr, desc, *args)
         cur.wait_stream(side)
     if rc != 0:
         h.check(rc, what)
@@ -602,7 +618,26 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class RMSNormalization(Operator):
+def _layout(t):
+    """What a call's checks and descriptor depend on: never where the elements are."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+class _Described:
+    """Operators whose checks and descriptors are kept from call to call, by the layout of the inputs."""
+
+    def _described(self, handle, make, *tensors):
+        key = (handle.device, *map(_layout, tensors))
+        kept = self.__dict__.setdefault("_kept", {})
+        got = kept.get(key)
+        if got is None:
+            if len(kept) >= 64:
+                kept.clear()
+            got = kept[key] = make(handle, *tensors)
+        return got
+
+
+class RMSNormalization(_Described, Operator):
     """ONNX RMSNormalization (opset 23) over the last axis.  Not in the reference registry.
 
     compute([x, scale], ctx, residual=None) returns [y], or with ``quantize`` [q, q_scale]: e4m3
@@ -632,9 +667,7 @@ class RMSNormalization(Operator):
             type(self).from_node(node)._check_axis(len(x))
         return [x]
 
-    def compute(self, inputs, ctx, residual=None):
-        x, w = inputs[0], inputs[1]
-        h = ctx.handle
+    def _describe(self, h, x, w, residual):
         what = "RMSNormalization"
         _check_device(h, what, x, w, residual)
         d = C.RmsNormDesc()
@@ -645,30 +678,38 @@ class RMSNormalization(Operator):
         lead, cols = tuple(x.shape[:-1]), x.shape[-1]
         if w.dim() != 1 or w.shape[0] != cols or not w.is_contiguous():
             raise ValidationError(C.ERR_VALIDATION, f"{what}: expected a contiguous scale of {cols} elements")
-        total = None
         if residual is not None:
             if residual.shape != x.shape or residual.dtype != x.dtype:
                 raise ValidationError(C.ERR_VALIDATION, f"{what}: the residual must have x's shape and type")
             d.ldr = _row_stride(residual, what)
-            total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d.rows, d.cols = math.prod(lead), cols
+        rows = math.prod(lead)
+        d.rows, d.cols = rows, cols
         d.epsilon = self.epsilon
-        qs = None
+        d.out_type = d.type
         if self.quantize:
             d.out_type = C.TYPE_E4M3
-            blocks = (cols + _QBLOCK - 1) // _QBLOCK
-            y, d.ldy = _stored_rows(lead, cols, x.device)
-            qs = _stored_scales(lead, d.rows, blocks, x.device)
-            d.y_scale_row, d.y_scale_block = 1, max(1, d.rows)
-        else:
-            d.out_type = d.type
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _launch(h, what, C.lib().onnxb200_rmsnorm, d, _ptr(x), _ptr(residual), _ptr(w), _ptr(total), _ptr(y), _ptr(qs))
+            d.ldy = _stored_stride(cols)
+            d.y_scale_row, d.y_scale_block = 1, max(1, rows)
+        blocks = (cols + _QBLOCK - 1) // _QBLOCK
+        same = _dense(x.shape, x.dtype)
+        return (d, ctypes.byref(d), _stored_rows(lead, cols) if self.quantize else same,
+                _stored_scales(lead, rows, blocks) if self.quantize else None, same if residual is not None else None)
+
+    def compute(self, inputs, ctx, residual=None):
+        x, w = inputs[0], inputs[1]
+        h = ctx.handle
+        _, desc, y_spec, qs_spec, sum_spec = self._described(h, self._describe, x, w, residual)
+        dev = x.device
+        y = _new(y_spec, dev)
+        qs = _new(qs_spec, dev) if qs_spec else None
+        total = _new(sum_spec, dev) if sum_spec else None
+        _launch(h, "RMSNormalization", C.lib().onnxb200_rmsnorm, desc, x.data_ptr(), _ptr(residual), w.data_ptr(),
+                _ptr(total), y.data_ptr(), _ptr(qs))
         out = [y] if qs is None else [y, qs]
         return out if total is None else out + [total]
 
 
-class QuantizeBlocks(Operator):
+class QuantizeBlocks(_Described, Operator):
     """e4m3 values and fp32 scales of a matrix: compute([x], ctx) returns [q, scale].  block_rows = 1
     gives one scale for every 128 columns of a row (activations, any leading dims), block_rows = 128
     one for 128 rows by 128 columns (weights, 2-D).  Not in the reference registry."""
@@ -691,9 +732,7 @@ class QuantizeBlocks(Operator):
         blocks = (x[-1] + _QBLOCK - 1) // _QBLOCK
         return [list(x), list(x[:-1]) + [blocks] if br == 1 else [(x[0] + _QBLOCK - 1) // _QBLOCK, blocks]]
 
-    def compute(self, inputs, ctx):
-        x = inputs[0]
-        h = ctx.handle
+    def _describe(self, h, x):
         what = "QuantizeBlocks"
         _check_device(h, what, x)
         d = C.QuantizeDesc()
@@ -702,21 +741,26 @@ class QuantizeBlocks(Operator):
         if self.block_rows != 1 and x.dim() != 2:
             raise ValidationError(C.ERR_VALIDATION, f"{what}: weights must be 2-D")
         lead, cols = tuple(x.shape[:-1]), x.shape[-1]
-        d.rows, d.cols = math.prod(lead), cols
+        rows, blocks = math.prod(lead), (cols + _QBLOCK - 1) // _QBLOCK
+        d.rows, d.cols, d.ldq = rows, cols, _stored_stride(cols)
         d.block_rows = self.block_rows
-        blocks = (cols + _QBLOCK - 1) // _QBLOCK
-        q, d.ldq = _stored_rows(lead, cols, x.device)
         if self.block_rows == 1:
-            s = _stored_scales(lead, d.rows, blocks, x.device)
-            d.scale_row, d.scale_block = 1, max(1, d.rows)
+            d.scale_row, d.scale_block = 1, max(1, rows)
         else:
-            s = torch.empty(((x.shape[0] + _QBLOCK - 1) // _QBLOCK, blocks), dtype=torch.float32, device=x.device)
             d.scale_row, d.scale_block = max(1, blocks), 1
-        _launch(h, what, C.lib().onnxb200_quantize_blocks, d, _ptr(x), _ptr(q), _ptr(s))
+        return (d, ctypes.byref(d), _stored_rows(lead, cols), _stored_scales(lead, rows, blocks) if self.block_rows == 1 else
+                _dense(((rows + _QBLOCK - 1) // _QBLOCK, blocks), torch.float32))
+
+    def compute(self, inputs, ctx):
+        x = inputs[0]
+        h = ctx.handle
+        _, desc, q_spec, s_spec = self._described(h, self._describe, x)
+        q, s = _new(q_spec, x.device), _new(s_spec, x.device)
+        _launch(h, "QuantizeBlocks", C.lib().onnxb200_quantize_blocks, desc, x.data_ptr(), q.data_ptr(), s.data_ptr())
         return [q, s]
 
 
-class MatMulBlockScaled(Operator):
+class MatMulBlockScaled(_Described, Operator):
     """y = A . B^T of e4m3 operands with a scale for every block of 128: compute([a, a_scale, b,
     b_scale, bias?], ctx) returns [y].  a is [..., k] with a_scale [..., ceil(k / 128)], b is
     [n, k] with b_scale [ceil(n / 128), ceil(k / 128)] (QuantizeBlocks(128)), bias fp32 [n]; y is
@@ -742,10 +786,7 @@ class MatMulBlockScaled(Operator):
         a, b = input_shapes[0], input_shapes[2]
         return [None if a is None or b is None else list(a[:-1]) + [b[0]]]
 
-    def compute(self, inputs, ctx):
-        a, a_scale, b, b_scale = inputs[:4]
-        bias = inputs[4] if len(inputs) > 4 else None
-        h = ctx.handle
+    def _describe(self, h, a, a_scale, b, b_scale, bias):
         what = "MatMulBlockScaled"
         _check_device(h, what, a, a_scale, b, b_scale, bias)
         if a.dtype != _E4M3 or b.dtype != _E4M3:
@@ -757,16 +798,32 @@ class MatMulBlockScaled(Operator):
             raise ValidationError(C.ERR_VALIDATION, f"Incompatible shapes for {what}: {list(a.shape)} and {list(b.shape)}")
         n, k = b.shape
         m = math.prod(a.shape[:-1])
-        blocks = (k + _QBLOCK - 1) // _QBLOCK
+        blocks, rows_b = (k + _QBLOCK - 1) // _QBLOCK, (n + _QBLOCK - 1) // _QBLOCK
         if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
             raise ValidationError(C.ERR_VALIDATION, f"{what}: expected a contiguous float32 bias of {n} elements")
         d.m, d.n, d.k = m, n, k
-        a_scale, d.a_scale_row, d.a_scale_block = _scale_strides(a_scale, m, blocks, what)
-        b_scale, d.b_scale_row, d.b_scale_block = _scale_strides(b_scale, (n + _QBLOCK - 1) // _QBLOCK, blocks, what)
+        # scales that are not addressable by two strides are laid out anew on every call
+        lay = []
+        for s, rows in ((a_scale, m), (b_scale, rows_b)):
+            t, sr, sb = _scale_strides(s, rows, blocks, what)
+            lay += [sr, sb, rows if t.data_ptr() != s.data_ptr() else None]
+        d.a_scale_row, d.a_scale_block, copy_a, d.b_scale_row, d.b_scale_block, copy_b = lay
         d.out_type = _TYPE[self.dtype]
         d.flags = C.EPI_RELU if self.relu else 0
-        y = torch.empty((*a.shape[:-1], n), dtype=self.dtype, device=a.device)
-        _launch(h, what, C.lib().onnxb200_matmul_blocks, d, _ptr(a), _ptr(a_scale), _ptr(b), _ptr(b_scale), _ptr(bias), _ptr(y))
+        return d, ctypes.byref(d), _dense((*a.shape[:-1], n), self.dtype), copy_a, copy_b, blocks
+
+    def compute(self, inputs, ctx):
+        a, a_scale, b, b_scale = inputs[:4]
+        bias = inputs[4] if len(inputs) > 4 else None
+        h = ctx.handle
+        _, desc, y_spec, copy_a, copy_b, blocks = self._described(h, self._describe, a, a_scale, b, b_scale, bias)
+        if copy_a is not None:
+            a_scale = _scale_strides(a_scale, copy_a, blocks, self.op_type)[0]
+        if copy_b is not None:
+            b_scale = _scale_strides(b_scale, copy_b, blocks, self.op_type)[0]
+        y = _new(y_spec, a.device)
+        _launch(h, "MatMulBlockScaled", C.lib().onnxb200_matmul_blocks, desc, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
+                b_scale.data_ptr(), _ptr(bias), y.data_ptr())
         return [y]
 
 

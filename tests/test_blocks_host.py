@@ -134,16 +134,19 @@ def test_row_stride(ob):
 
 
 def test_stored_layouts(ob):
-    q, ld = ob.ops._stored_rows((3, 2), 33, "cpu")
-    assert q.shape == (3, 2, 33) and ld == 48 and ob.ops._row_stride(q, "q") == 48
-    q, ld = ob.ops._stored_rows((), 64, "cpu")
-    assert q.shape == (64,) and ld == 64
-    for lead, rows in (((3, 2), 6), ((6,), 6), ((), 1), ((1,), 1)):
-        s = ob.ops._stored_scales(lead, rows, 5, "cpu")
+    new = lambda spec: ob.ops._new(spec, "cpu")
+    q = new(ob.ops._stored_rows((3, 2), 33))
+    assert q.shape == (3, 2, 33) and ob.ops._stored_stride(33) == 48 and ob.ops._row_stride(q, "q") == 48
+    q = new(ob.ops._stored_rows((), 64))
+    assert q.shape == (64,) and ob.ops._stored_stride(64) == 64
+    for shape in ((), (4,), (3, 0), (0, 3), (2, 3, 4)):
+        assert new(ob.ops._dense(shape, torch.float32)).stride() == torch.empty(shape).stride()
+    for lead, rows in (((3, 2), 6), ((6,), 6), ((), 1), ((1,), 1), ((0,), 0)):
+        s = new(ob.ops._stored_scales(lead, rows, 5))
         assert s.shape == (*lead, 5)
         back, sr, sb = ob.ops._scale_strides(s, rows, 5, "s")
         assert back.data_ptr() == s.data_ptr()  # read in place, never copied
-        assert (rows == 1 or sr == 1) and sb == rows
+        assert rows <= 1 or (sr, sb) == (1, rows)
 
 
 def test_scale_strides(ob):
