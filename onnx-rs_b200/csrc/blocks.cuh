@@ -93,6 +93,25 @@ int launch_pdl(void (*kernel)(P...), unsigned grid, unsigned threads, size_t sme
   return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// The low two bytes of q as two fp16 (exact; NaN stays NaN).
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t q) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)q));
+  return r;
+}
+// c + a.lo * b.lo + a.hi * b.hi of two fp16 pairs, each step one fp32 rounding.
+__device__ __forceinline__ float fma_f16x2(uint32_t a, uint32_t b, float c) {
+  float d;
+  asm("{\n\t.reg .b16 al, ah, bl, bh;\n\t"
+      "mov.b32 {al, ah}, %1;\n\t"
+      "mov.b32 {bl, bh}, %2;\n\t"
+      "fma.rn.f32.f16 %0, al, bl, %3;\n\t"
+      "fma.rn.f32.f16 %0, ah, bh, %0;\n\t}"
+      : "=&f"(d)
+      : "r"(a), "r"(b), "f"(c));
+  return d;
+}
+
 // Calls f with a null pointer of the element type `t` (F32, F16 or BF16).
 template <typename F>
 auto with_type(int t, F f) {

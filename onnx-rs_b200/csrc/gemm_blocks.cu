@@ -89,6 +89,112 @@ __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlo
     }
 }
 
+// ---------------------------------------------------------------- one or two rows
+// A single decoding step reads every byte of b once for a handful of products per
+// byte: CUDA cores keep up with HBM, without the tensor core's set-up or a join over
+// CTAs.  A warp takes two rows of b, 16 bytes per lane and load, eight loads in
+// flight; a is turned into fp16 (exact) once per block, and products are fused into
+// fp32 sums of 16, which are scaled and added.
+constexpr int kVecWarps = 8, kVecRows = 2, kVecUnroll = 4;
+constexpr int kVecMaxSmem = 100 * 1024;  // two blocks per SM; longer rows of a go to the tensor cores
+template <typename T, int M>
+__global__ void __launch_bounds__(kVecWarps * 32) matmul_blocks_vec_kernel(const MatmulBlocksArgs p) {
+  extern __shared__ uint4 va[];  // [M][2][chunks] eight fp16 of a; then [M][blocks] scales
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = (p.k + 15) / 16, kbs = (p.k + kQBlock - 1) / kQBlock;
+  float* sc = reinterpret_cast<float*>(va + M * 2 * chunks);
+  const int n0 = (blockIdx.x * kVecWarps + warp) * kVecRows;
+  pdl_begin();
+
+  // 16 bytes of a row of k, zeros behind its end
+  auto load16 = [&](const uint8_t* row, int c) {
+    if (c * 16 + 16 <= p.k) return *reinterpret_cast<const uint4*>(row + c * 16);
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = c * 16; i < p.k; ++i) w[(i & 15) >> 2] |= (uint32_t)row[i] << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  // Steps of 512 k's (16 bytes a lane) that lie whole in a row: a ring of kVecUnroll
+  // of them is in flight, refilled as each is used up.
+  const int steps = p.k / 512;
+  const uint8_t* rows[kVecRows];
+#pragma unroll
+  for (int r = 0; r < kVecRows; ++r) rows[r] = p.b + (int64_t)min(n0 + r, p.n - 1) * p.ldb;
+  uint4 w[kVecUnroll][kVecRows];
+  auto fetch = [&](int u, int step) {
+#pragma unroll
+    for (int r = 0; r < kVecRows; ++r) w[u][r] = *reinterpret_cast<const uint4*>(rows[r] + step * 512 + lane * 16);
+  };
+#pragma unroll
+  for (int u = 0; u < kVecUnroll; ++u)
+    if (u < steps) fetch(u, u);
+  for (int i = threadIdx.x; i < M * chunks; i += kVecWarps * 32) {
+    const int m = i / chunks, c = i - m * chunks;
+    const uint4 q = m < p.m ? load16(p.a + m * p.lda, c) : make_uint4(0, 0, 0, 0);
+    va[(m * 2) * chunks + c] = make_uint4(e4m3x2_to_f16x2(q.x), e4m3x2_to_f16x2(q.x >> 16), e4m3x2_to_f16x2(q.y),
+                                          e4m3x2_to_f16x2(q.y >> 16));
+    va[(m * 2 + 1) * chunks + c] = make_uint4(e4m3x2_to_f16x2(q.z), e4m3x2_to_f16x2(q.z >> 16), e4m3x2_to_f16x2(q.w),
+                                              e4m3x2_to_f16x2(q.w >> 16));
+  }
+  const float* bs = p.bs + (int64_t)(blockIdx.x * (kVecWarps * kVecRows) / kQBlock) * p.bs_row;
+  for (int i = threadIdx.x; i < M * kbs; i += kVecWarps * 32) {
+    const int m = i / kbs, kb = i - m * kbs;
+    sc[i] = m < p.m ? p.as[m * p.as_row + kb * p.as_block] * bs[kb * p.bs_block] : 0.f;
+  }
+  __syncthreads();
+
+  float acc[kVecRows][M] = {};
+  auto add = [&](const uint4 (&q4)[kVecRows], int c) {  // chunk c of 16 k's
+    uint32_t h[kVecRows][8];
+#pragma unroll
+    for (int r = 0; r < kVecRows; ++r) {
+      const uint32_t q[4] = {q4[r].x, q4[r].y, q4[r].z, q4[r].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[r][i] = e4m3x2_to_f16x2(i & 1 ? q[i / 2] >> 16 : q[i / 2]);
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const uint4 lo = va[(m * 2) * chunks + c], hi = va[(m * 2 + 1) * chunks + c];
+      const uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      const float s = sc[m * kbs + c / 8];
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r) {
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d = fma_f16x2(x[i], h[r][i], d);
+        acc[r][m] = fmaf(d, s, acc[r][m]);
+      }
+    }
+  };
+  for (int s0 = 0; s0 < steps; s0 += kVecUnroll) {
+#pragma unroll
+    for (int u = 0; u < kVecUnroll; ++u) {
+      if (s0 + u >= steps) break;
+      add(w[u], (s0 + u) * 32 + lane);
+      if (s0 + u + kVecUnroll < steps) fetch(u, s0 + u + kVecUnroll);
+    }
+  }
+  if (steps * 32 + lane < chunks) {
+    uint4 q[kVecRows];
+#pragma unroll
+    for (int r = 0; r < kVecRows; ++r) q[r] = load16(rows[r], steps * 32 + lane);
+    add(q, steps * 32 + lane);
+  }
+#pragma unroll
+  for (int r = 0; r < kVecRows; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      float v = acc[r][m];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      const int n = n0 + r;
+      if (lane == r * M + m && n < p.n && m < p.m) {
+        if (p.bias) v += p.bias[n];
+        if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays NaN
+        static_cast<T*>(p.y)[m * p.ldy + n] = from_f32<T>(v);
+      }
+    }
+}
+
 // ---------------------------------------------------------------- few rows
 // Tokens are the MMA's N and weights its M: a tile is 128 rows of b by BN rows of
 // a, so a handful of tokens wastes no tensor-core rows and y's columns (n) lie
@@ -98,10 +204,10 @@ __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlo
 // workspace, the same bits every time.
 template <int BN>
 struct RowsLayout {
-  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
+  static constexpr int kStages = BN == 16 ? 5 : 4;          // two CTAs per SM: at most 113 KB each
   static constexpr int kW = 128 * 128, kX = BN * 128, kStage = kW + kX;
-  static constexpr int kBufs = BN == 128 ? 2 : 4;          // TMEM accumulators
-  static constexpr int kCols = BN * kBufs;                  // 64, 128, 256, 256
+  static constexpr int kCols = 256;                         // two CTAs per SM share 512
+  static constexpr int kBufs = kCols / BN;                  // accumulators: the MMAs rarely wait for the epilogue
   static constexpr int kChunk = 1024 / BN;                  // k-blocks whose scales are staged at once
   static constexpr int kOffScale = kStages * kStage;        // 2 x kChunk x BN floats
   static constexpr int kOffBar = kOffScale + 2 * 4096;
@@ -184,7 +290,6 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       }
     };
     load_scales(0);
-    bool ok = true;
     const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
     for (int it = 0; it < nkb; ++it) {
       const int c = it / CH;
@@ -193,34 +298,30 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         // the buffer's readers of chunk c - 2 passed the barrier of chunk c - 1
 #pragma unroll
         for (int i = 0; i < 8; ++i) buf[i * 128 + threadIdx.x] = nxt[i];
-        ok = named_bar_and(ok, 128);
+        named_bar_sync(128);
         if ((c + 1) * CH < nkb) load_scales(c + 1);
       }
-      // after a wait that gave up, the warp only keeps the barriers above going
       const int b = it % NB;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full(b), (it / NB) & 1, abort_flag, p.status));
-      if (!ok) continue;
+      bar_wait(acc_full(b), (it / NB) & 1, abort_flag, p.status);
+      __syncwarp();
       tc_fence_after();
+      uint32_t r[BN / 16][16];
+#pragma unroll
+      for (int g = 0; g < BN / 16; ++g) tmem_ld_32x32b_x16(lane_addr + b * BN + g * 16, r[g]);
       const float4* s4 = reinterpret_cast<const float4*>(buf + it % CH * BN);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(b));
 #pragma unroll
-      for (int g = 0; g < BN / 16; ++g) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(lane_addr + b * BN + g * 16, r);
-        tmem_ld_wait();
-        if (g == BN / 16 - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty(b));
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 s = s4[g * 4 + q];
-          float* a = acc + g * 16 + q * 4;
-          a[0] = fmaf(__uint_as_float(r[q * 4]), s.x, a[0]);
-          a[1] = fmaf(__uint_as_float(r[q * 4 + 1]), s.y, a[1]);
-          a[2] = fmaf(__uint_as_float(r[q * 4 + 2]), s.z, a[2]);
-          a[3] = fmaf(__uint_as_float(r[q * 4 + 3]), s.w, a[3]);
-        }
+      for (int q = 0; q < BN / 4; ++q) {
+        const float4 s = s4[q];
+        const uint32_t* d = r[q / 4] + q % 4 * 4;
+        float* a = acc + q * 4;
+        a[0] = fmaf(__uint_as_float(d[0]), s.x, a[0]);
+        a[1] = fmaf(__uint_as_float(d[1]), s.y, a[1]);
+        a[2] = fmaf(__uint_as_float(d[2]), s.z, a[2]);
+        a[3] = fmaf(__uint_as_float(d[3]), s.w, a[3]);
       }
     }
   } else if (warp == 4) {
@@ -241,26 +342,26 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     __syncwarp();
   } else {
     constexpr uint32_t idesc = make_idesc(0, 128, BN);
-    if (lane == 0) {
-      int it = 0;
-      for (; it < nkb; ++it) {
-        const int s = it % ST, b = it % NB;
-        if (!mbar_wait(acc_empty(b), ((it / NB) & 1) ^ 1, abort_flag, p.status)) break;
-        if (!mbar_wait(full(s), (it / ST) & 1, abort_flag, p.status)) break;
-        tc_fence_after();
-        const uint64_t dw = smem_desc_sw128(base + s * L::kStage);
-        const uint64_t dx = smem_desc_sw128(base + s * L::kStage + L::kW);
+    const bool leader = elect_one();
+    for (int it = 0; it < nkb; ++it) {
+      const int s = it % ST, b = it % NB;
+      const uint64_t dw = smem_desc_sw128(base + s * L::kStage);
+      const uint64_t dx = smem_desc_sw128(base + s * L::kStage + L::kW);
+      if (it >= NB) bar_wait(acc_empty(b), ((it / NB) & 1) ^ 1, abort_flag, p.status);
+      bar_wait(full(s), (it / ST) & 1, abort_flag, p.status);
+      tc_fence_after();
+      if (leader) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           tc_mma_e4m3<1>(tmem + b * BN, dw + (uint64_t)(kk * 2), dx + (uint64_t)(kk * 2), idesc, kk ? 1u : 0u);
         tc_commit(empty(s));
         tc_commit(acc_full(b));
       }
-      if (it) {  // every MMA has completed before TMEM is freed
-        tc_commit(drain);
-        volatile int no_abort = 0;
-        mbar_wait(drain, 0, &no_abort, p.status);
-      }
+    }
+    if (leader) {  // every MMA has completed before TMEM is freed
+      tc_commit(drain);
+      volatile int no_abort = 0;
+      mbar_wait(drain, 0, &no_abort, p.status);
     }
     __syncwarp();
   }
@@ -694,6 +795,16 @@ int opt_in(int bytes) {
   return (int)e;
 }
 
+template <typename T, int M>
+int launch_vec(const MatmulBlocksArgs& a, size_t smem, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    const int rc = opt_in<matmul_blocks_vec_kernel<T, M>>(kVecMaxSmem);
+    if (rc) return rc;
+  }
+  const unsigned per = kVecWarps * kVecRows;
+  return launch_pdl(matmul_blocks_vec_kernel<T, M>, (a.n + per - 1) / per, kVecWarps * 32, smem, st, a);
+}
+
 template <typename T, int BN>
 int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
   using L = RowsLayout<BN>;
@@ -773,11 +884,16 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       const int64_t wide = (tm * ((a.n + 255) / 256) + pairs - 1) / pairs, narrow = (tm * ((a.n + 127) / 128) + pairs - 1) / pairs;
       return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
     }
-    // split k until about one CTA per SM runs, at least 4 blocks each (1 x 4096 x
-    // 4096: 15.3, 11.6, 9.2 and 17.0 us with 1, 2, 4 and 8 CTAs per tile)
+    const size_t vec_smem = (size_t)a.m * ((a.k + 15) / 16 * 32 + kbs * 4);
+    if (a.m <= 2 && vec_smem <= kVecMaxSmem)
+      return a.m == 1 ? launch_vec<T, 1>(a, vec_smem, st) : launch_vec<T, 2>(a, vec_smem, st);
+    // Split k over CTAs until they fill the GPU's SMs once or twice, two blocks each at
+    // least; the first split also pays for the clusters (16 x 4096 x 4096 with 32
+    // tiles: 12.9, 10.8, 8.9 and 8.7 us with 1, 2, 4 and 8 CTAs a tile; 16 x 14336 x
+    // 4096 with 112: 15.1, 16.4, 19.9; 17 x 1000 x 2048 with 8: 9.1, 9.2, 7.2, 5.9).
     const int tiles = (a.n + 127) / 128;
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= num_sms && kbs >= split * 2 * 4) split *= 2;
+    int split = tiles * 4 <= num_sms * 3 && kbs >= 4 ? 2 : 1;
+    while (split > 1 && split < 8 && tiles * split <= num_sms && kbs >= split * 4) split *= 2;
     return a.m <= 16 ? launch_rows<T, 16>(a, split, st) : launch_rows<T, 32>(a, split, st);
   });
 }
