@@ -437,9 +437,9 @@ struct PairLayout {
   static constexpr int kHalves = BN / 128;
   static constexpr int kBufs = 4 / kHalves;            // accumulators per half: 512 TMEM columns in all
   static constexpr int kA = 128 * 128, kB = BN / 2 * 128, kStage = kA + kB;
-  static constexpr int kStages = BN == 256 ? 5 : 6;
-  static constexpr int kRB = 64, kOutBufs = 3;         // staging: rows of 64 bytes, three buffers of 32 rows per warp
-  static constexpr int kOutWarp = kOutBufs * 32 * kRB;
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kOutBufs = 2;                   // staging: 32 rows of 128 bytes, two per warp
+  static constexpr int kOutWarp = kOutBufs * 32 * 128;
   static constexpr int kOffOut = kStages * kStage;
   static constexpr int kOffScale = kOffOut + kPairEpiWarps * kOutWarp;  // two groups: [halves][128] rows of four blocks
   static constexpr int kScaleGroup = 4 * kHalves * 128;
@@ -570,70 +570,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tile_at(t, mt, nt);
       const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
       const int col0 = nt * BN + half * 128 + within;
-      constexpr int ES = sizeof(T), CPR = L::kRB / ES;  // columns of a staging row
-      const uint32_t stage0 = base + L::kOffOut + warp * L::kOutWarp + lane * 64;
-      const uint32_t swz = (lane >> 1) & 3;
+      constexpr int ES = sizeof(T), PER = 16 / ES, CPR = 128 / ES;  // columns of a 16-byte unit, of a staging row
+      constexpr int NC = CW / CPR, OB = NC < L::kOutBufs ? NC : L::kOutBufs;
+      const uint32_t out = base + L::kOffOut + warp * L::kOutWarp;
 #pragma unroll
-      for (int c = 0; c < CW / CPR; ++c) {
-        if (lane == 0) bulk_wait_group_read<L::kOutBufs - 1>();  // the last store from this buffer has read it
+      for (int c0 = 0; c0 < NC; c0 += OB) {
+        if (lane == 0) bulk_wait_group_read<0>();  // the last stores have read the buffers
         __syncwarp();
-        const uint32_t mine = stage0 + c % L::kOutBufs * (32 * L::kRB);
+        auto stage = [&](auto extras) {  // with bias and Relu, or without either
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          constexpr int PER = 16 / ES;  // columns of a unit
-          float f[PER];
+          for (int c = c0; c < c0 + OB; ++c) {
+            const uint32_t mine = out + (c - c0) * 4096 + lane * 128;
 #pragma unroll
-          for (int q = 0; q < PER; q += 2) {
-            const float2 v = unpack_f2(acc[(c * CPR + u * PER + q) / 2]);
-            f[q] = v.x;
-            f[q + 1] = v.y;
+            for (int u = 0; u < 8; ++u) {
+              float f[PER];
+#pragma unroll
+              for (int q = 0; q < PER; q += 2) {
+                const float2 v = unpack_f2(acc[(c * CPR + u * PER + q) / 2]);
+                f[q] = v.x;
+                f[q + 1] = v.y;
+              }
+              if constexpr (decltype(extras)::value) {
+                const int j0 = col0 + c * CPR + u * PER;
+#pragma unroll
+                for (int q = 0; q < PER; ++q) {
+                  if (p.bias) f[q] += p.bias[min(j0 + q, p.n - 1)];
+                  if (p.relu) f[q] = f[q] < 0.f ? 0.f : f[q];  // NaN stays NaN
+                }
+              }
+              uint32_t w[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if constexpr (ES == 4)
+                  w[q] = __float_as_uint(f[q]);
+                else
+                  w[q] = pack_rounded<T>(f[2 * q], f[2 * q + 1]);
+              }
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((u ^ (lane & 7)) * 16)), "r"(w[0]),
+                           "r"(w[1]), "r"(w[2]), "r"(w[3])
+                           : "memory");
+            }
           }
-          if (p.bias) {
-            const int j0 = col0 + c * CPR + u * PER;
-#pragma unroll
-            for (int q = 0; q < PER; ++q) f[q] += p.bias[min(j0 + q, p.n - 1)];
-          }
-          if (p.relu) {
-#pragma unroll
-            for (int q = 0; q < PER; ++q) f[q] = f[q] < 0.f ? 0.f : f[q];  // NaN stays NaN
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if constexpr (ES == 4)
-              w[q] = __float_as_uint(f[q]);
-            else
-              w[q] = pack_rounded<T>(f[2 * q], f[2 * q + 1]);
-          }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((u ^ swz) * 16)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                       "r"(w[3])
-                       : "memory");
-        }
-        const int colc = col0 + c * CPR;
-        const uint32_t out = mine - lane * 64;
+        };
+        if (p.bias || p.relu)
+          stage(std::true_type{});
+        else
+          stage(std::false_type{});
         if (tma_out) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (row0 < p.m && colc < p.n) tma_store_2d(&tm_y, colc, row0, out);
+#pragma unroll
+            for (int c = c0; c < c0 + OB; ++c)
+              if (row0 < p.m && col0 + c * CPR < p.n) tma_store_2d(&tm_y, col0 + c * CPR, row0, out + (c - c0) * 4096);
             bulk_commit_group();
           }
         } else {
           __syncwarp();
-          const int u = lane & 3, col = colc + u * (16 / ES);
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
-            const int rr = q * 8 + (lane >> 2);
+          for (int q = 0; q < OB * 8; ++q) {
+            const int rr = q % 8 * 4 + (lane >> 3), u = lane & 7, col = col0 + (c0 + q / 8) * CPR + u * PER;
             uint32_t w[4];
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                         : "r"(out + rr * 64 + ((u ^ ((rr >> 1) & 3)) * 16))
+                         : "r"(out + q / 8 * 4096 + rr * 128 + ((u ^ (rr & 7)) * 16))
                          : "memory");
             if (row0 + rr < p.m) {
               T* dst = static_cast<T*>(p.y) + (row0 + rr) * p.ldy + col;
               const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
-              for (int k = 0; k < 16 / ES; ++k)
+              for (int k = 0; k < PER; ++k)
                 if (col + k < p.n) dst[k] = e[k];
             }
           }
@@ -830,15 +836,15 @@ int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
   return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_rows_kernel<T, BN>, a, w, x, split, x_tiles);
 }
 
-// Boxes of 32 rows by `box_bytes` of y, for the stores; false where TMA cannot write.
+// Boxes of 32 rows by 128 bytes of y, for the stores; false where TMA cannot write.
 template <typename T>
-bool encode_out(const MatmulBlocksArgs& a, int box_bytes, CUtensorMap* map) {
+bool encode_out(const MatmulBlocksArgs& a, CUtensorMap* map) {
   EncodeFn fn = encode_fn();
   if (!fn || (reinterpret_cast<uintptr_t>(a.y) & 15) || a.ldy * sizeof(T) % 16) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)a.n, (cuuint64_t)a.m}, strides[1] = {(cuuint64_t)a.ldy * sizeof(T)};
-  const cuuint32_t boxes[2] = {(cuuint32_t)(box_bytes / sizeof(T)), 32}, es[2] = {1, 1};
+  const cuuint32_t boxes[2] = {(cuuint32_t)(128 / sizeof(T)), 32}, es[2] = {1, 1};
   return fn(map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a.y, dims, strides,
-            boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -848,7 +854,7 @@ int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st) {
   CUtensorMap ma, mb, my{};
   if (!encode_rows(a.a, a.m, a.k, a.lda, 128, &ma) || !encode_rows(a.b, a.n, a.k, a.ldb, 64, &mb))
     return (int)cudaErrorInvalidValue;
-  const int tma_out = encode_out<T>(a, L::kRB, &my);
+  const int tma_out = encode_out<T>(a, &my);
   int rc = opt_in<matmul_blocks_pair_kernel<T, BN>>(L::kBytes);
   if (rc) return rc;
   const int tiles = ((a.m + 255) / 256) * ((a.n + BN - 1) / BN);
