@@ -343,10 +343,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   } else {
     constexpr uint32_t idesc = make_idesc(0, 128, BN);
     const bool leader = elect_one();
+    const uint64_t dw0 = smem_desc_sw128(base);  // a descriptor's address counts 16-byte units
     for (int it = 0; it < nkb; ++it) {
       const int s = it % ST, b = it % NB;
-      const uint64_t dw = smem_desc_sw128(base + s * L::kStage);
-      const uint64_t dx = smem_desc_sw128(base + s * L::kStage + L::kW);
+      const uint64_t dw = dw0 + (uint64_t)(s * (L::kStage >> 4)), dx = dw + (L::kW >> 4);
       if (it >= NB) bar_wait(acc_empty(b), ((it / NB) & 1) ^ 1, abort_flag, p.status);
       bar_wait(full(s), (it / ST) & 1, abort_flag, p.status);
       tc_fence_after();
@@ -683,12 +683,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     constexpr uint32_t idesc = make_idesc(0, 256, 128);
     if (rank == 0) {
       const bool leader = elect_one();
+      const uint64_t da0 = smem_desc_sw128(base);  // a descriptor's address counts 16-byte units
       int s = 0, buf = 0;
       uint32_t sp = 0, bp = 1;  // parities: of the stage's use, of the buffer's release
       const int total = nkb * ((tiles - (int)(blockIdx.x / 2) + pairs - 1) / pairs);
       for (int it = 0; it < total; ++it) {
-        const uint64_t da = smem_desc_sw128(base + s * L::kStage);
-        const uint64_t db = smem_desc_sw128(base + s * L::kStage + L::kA);
+        const uint64_t da = da0 + (uint64_t)(s * (L::kStage >> 4)), db = da + (L::kA >> 4);
         bar_wait(full(s), sp, abort_flag, p.status);
 #pragma unroll
         for (int hf = 0; hf < NH; ++hf) {
