@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "blocks.h"
@@ -69,6 +70,20 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
 }
 __device__ __forceinline__ float from_e4m3(uint8_t v) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+}
+
+// The shared-memory opt-in is a per-device attribute of a kernel, set once: to the
+// most that any call asks for, so that calls on several threads agree.
+template <auto KERNEL>
+int opt_in(int bytes) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> done[kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return (int)cudaErrorInvalidDevice;
+  if (done[dev].load(std::memory_order_relaxed)) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done[dev].store(true, std::memory_order_relaxed);
+  return (int)e;
 }
 
 // Programmatic dependent launch: the kernel's blocks may start while the previous

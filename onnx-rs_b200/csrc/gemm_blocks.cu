@@ -15,9 +15,10 @@
 namespace ob2 {
 namespace {
 // Waits without a result: after a wait that gave up (status and abort flag set) the
-// ones behind it return within a millisecond each, and the kernel runs on, over whatever its buffers
-// hold, to its end.  No branch on the outcome, and polling before sleeping: both sit
-// on the round trip between the MMAs and the epilogue that bounds the products.
+// ones behind it return within a millisecond each, and the kernel runs on, over
+// whatever its buffers hold, to its end.  No branch on the outcome, and polling before
+// sleeping: both sit on the round trip between the MMAs and the epilogue that bounds
+// the products.
 __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
   for (int i = 0; i < 64; ++i)
     if (mbar_try_wait(bar, parity)) return;
@@ -90,11 +91,14 @@ __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlo
 }
 
 // ---------------------------------------------------------------- one or two rows
-// A single decoding step reads every byte of b once for a handful of products per
-// byte: CUDA cores keep up with HBM, without the tensor core's set-up or a join over
-// CTAs.  A warp takes two rows of b, 16 bytes per lane and load, eight loads in
+// A single decoding step reads every byte of b once for one or two products per
+// byte: CUDA cores nearly keep up with HBM, without the tensor core's set-up or a join
+// over CTAs.  A warp takes two rows of b, 16 bytes per lane and load, eight loads in
 // flight; a is turned into fp16 (exact) once per block, and products are fused into
-// fp32 sums of 16, which are scaled and added.
+// fp32 sums of 16, which are scaled and added.  The mixed fp16 -> fp32 fused
+// multiply-adds run at a quarter of the fp32 rate: 1 x 4096 x 4096 takes 6.7 us (17
+// MB; 8.1 in the kernel for few rows), 1 x 8192 x 8192 15.4 us (4.4 TB/s), 2 x 4096 x
+// 4096 8.3 us, and four rows 10.9, more than below.
 constexpr int kVecWarps = 8, kVecRows = 2, kVecUnroll = 4;
 constexpr int kVecMaxSmem = 100 * 1024;  // two blocks per SM; longer rows of a go to the tensor cores
 template <typename T, int M>
@@ -196,12 +200,14 @@ __global__ void __launch_bounds__(kVecWarps * 32) matmul_blocks_vec_kernel(const
 }
 
 // ---------------------------------------------------------------- few rows
-// Tokens are the MMA's N and weights its M: a tile is 128 rows of b by BN rows of
-// a, so a handful of tokens wastes no tensor-core rows and y's columns (n) lie
-// along the lanes, whose stores are then contiguous.  The k range is split over
-// the CTAs of a cluster; each leaves its partial sums in shared memory, and the
-// sums are joined in rank order over distributed shared memory: one launch, no
-// workspace, the same bits every time.
+// Three to 32 rows of a.  They are the MMA's N and the weights its M: a tile is 128
+// rows of b by all rows of a (BN >= m), so a handful of tokens wastes no tensor-core
+// rows and y's columns (n) lie along the lanes, whose stores are then contiguous.
+// The k range is split over the CTAs of a cluster; each leaves its partial sums in
+// shared memory, and the sums are joined in rank order over distributed shared
+// memory: one launch, no workspace, the same bits every time.  Bound by HBM with
+// many weights (16 x 14336 x 4096, 59 MB: 15.1 us, 3.9 TB/s), by the start of its
+// CTAs and the join with few (16 x 4096 x 4096: 8.7 us, of which 2.6 are bytes).
 template <int BN>
 struct RowsLayout {
   static constexpr int kStages = BN == 16 ? 5 : 4;          // two CTAs per SM: at most 113 KB each
@@ -221,7 +227,7 @@ constexpr int kRowsThreads = 192;  // 4 epilogue warps, TMA, MMA
 template <typename T, int BN>
 __global__ void __launch_bounds__(kRowsThreads, 2)
     matmul_blocks_rows_kernel(const __grid_constant__ MatmulBlocksArgs p, const __grid_constant__ CUtensorMap tm_w,
-                              const __grid_constant__ CUtensorMap tm_x, int split, int x_tiles) {
+                              const __grid_constant__ CUtensorMap tm_x, int split) {
   using L = RowsLayout<BN>;
   constexpr int ST = L::kStages, NB = L::kBufs, CH = L::kChunk;
   extern __shared__ uint8_t smem_raw[];
@@ -266,8 +272,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   pdl_begin();
 
   const int rank = blockIdx.x % split;
-  const int tile = blockIdx.x / split;
-  const int n0 = tile / x_tiles * 128, m0 = tile % x_tiles * BN;
+  const int n0 = blockIdx.x / split * 128;
   const int kbs = (p.k + kQBlock - 1) / kQBlock;
   const int kb0 = (int)((int64_t)kbs * rank / split), kb1 = (int)((int64_t)kbs * (rank + 1) / split);
   const int nkb = kb1 - kb0;
@@ -285,7 +290,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int idx = i * 128 + threadIdx.x;
-        const int kb = kb0 + c * CH + idx / BN, m = m0 + idx % BN;
+        const int kb = kb0 + c * CH + idx / BN, m = idx % BN;
         nxt[i] = kb < kb1 && m < p.m ? p.as[m * p.as_row + kb * p.as_block] * bs[kb * p.bs_block] : 0.f;
       }
     };
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
         mbar_arrive_expect_tx(full(s), L::kStage);
         const uint32_t dst = base + s * L::kStage;
         tma_load_2d(dst, &tm_w, (kb0 + it) * kQBlock, n0, full(s));
-        tma_load_2d(dst + L::kW, &tm_x, (kb0 + it) * kQBlock, m0, full(s));
+        tma_load_2d(dst + L::kW, &tm_x, (kb0 + it) * kQBlock, 0, full(s));
       }
       // every copy has landed before the CTA may exit
       volatile int no_abort = 0;
@@ -374,8 +379,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 
   T* y = static_cast<T*>(p.y);
   const int n = n0 + (threadIdx.x & 127);
-  auto finish = [&](int j, float v, float bias) {
-    const int m = m0 + j;
+  auto finish = [&](int m, float v, float bias) {
     if (m < p.m && n < p.n) {
       v += bias;
       if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays NaN
@@ -425,6 +429,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 // scales of a and b and hands them over four blocks at a time.  Persistent: pairs
 // walk the tiles, and a tile's stores (TMA, from shared memory) run under the
 // next tile's loads and MMAs.
+//
+// What bounds it: at 256 x 256 a block of 128 k's takes 730 cycles, of which the
+// MMAs need 512 (a pure stream of them measured 512, at 1.4 GHz under the power cap
+// 3.3 PFLOP/s); the rest is the round trip MMA -> commit -> 8 reads of 16 TMEM
+// columns -> arrival on the leader, which two accumulators per half do not cover.
+// TMEM is full, and so are the registers: reads of 32 columns, or sixteen warps with
+// half the totals each, spilled and were slower (8192^3: 568 and 580 us against 490),
+// as were both halves in every warp (525) and asking barriers one block ahead (498).
+// 8192^3 bf16: 465-500 us, 2.2-2.4 PFLOP/s; 4096^3 62 us; 8192 x 8192 x 1024 74 us;
+// 200 x 8192 x 4096 (256 x 128 tiles, 36 MB) 15 us, its loop at 4.7 TB/s.
+//
 // 8 epilogue warps, then a warpgroup with the TMA, MMA and scale warps.  Launched
 // with 168 registers a thread (384 x 168 = 64512), split as 208 for the totals and
 // 88 for the rest (256 x 208 + 128 x 88 = 64512).
@@ -447,8 +462,9 @@ struct PairLayout {
   static constexpr int kBars = 2 * kStages + 13;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kBytes = kOffMisc + 16 + 1024;
-  static constexpr int kCW = BN * 4 / kPairEpiWarps;                   // columns per epilogue warp
+  static constexpr int kCW = BN * 4 / kPairEpiWarps;   // columns per epilogue warp
 };
+
 template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     matmul_blocks_pair_kernel(const __grid_constant__ MatmulBlocksArgs p, const __grid_constant__ CUtensorMap tm_a,
@@ -491,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     fence_mbarrier_init();
   }
   if (warp == kPairEpiWarps + 1) tmem_alloc_pair(smem_u32(tmem_slot), 512);
-  if (warp == kPairEpiWarps + 0 && lane == 0) {
+  if (warp == kPairEpiWarps && lane == 0) {
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
     if (tma_out) prefetch_tmap(&tm_y);
@@ -565,7 +581,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // Bias, Relu, rounding; then a warp's 32 rows go through its own staging
       // rows (swizzled as the TMA map wants them, which is also free of bank
       // conflicts) to TMA stores that clip the tile's edges; where TMA cannot
-      // write (y off the 16-byte grid), element by element.
+      // write (y, or its last column, off the 16-byte grid), element by element.
       int mt, nt;
       tile_at(t, mt, nt);
       const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
@@ -616,7 +632,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           stage(std::true_type{});
         else
           stage(std::false_type{});
-        if (tma_out) {
+        // a store's box is cut in units of 16 bytes: an edge inside one is written by elements
+        if (tma_out && (p.n % PER == 0 || col0 + (c0 + OB) * CPR <= p.n)) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -652,7 +669,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
-  if (warp == kPairEpiWarps + 0) {
+  if (warp == kPairEpiWarps) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
@@ -788,19 +805,6 @@ bool encode_rows(const uint8_t* q, int rows, int k, int64_t ld, int box, CUtenso
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The shared-memory opt-in is a per-device attribute of a kernel.
-template <auto KERNEL>
-int opt_in(int bytes) {
-  constexpr int kMaxDevices = 64;
-  static bool done[kMaxDevices] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return (int)cudaErrorInvalidDevice;
-  if (done[dev]) return 0;
-  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) done[dev] = true;
-  return (int)e;
-}
-
 template <typename T, int M>
 int launch_vec(const MatmulBlocksArgs& a, size_t smem, cudaStream_t st) {
   if (smem > 48 * 1024) {
@@ -819,9 +823,8 @@ int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
     return (int)cudaErrorInvalidValue;
   int rc = opt_in<matmul_blocks_rows_kernel<T, BN>>(L::kBytes);
   if (rc) return rc;
-  const int x_tiles = (a.m + BN - 1) / BN;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.n + 127) / 128) * x_tiles * split);
+  cfg.gridDim = dim3((unsigned)((a.n + 127) / 128) * split);
   cfg.blockDim = dim3(kRowsThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
@@ -833,7 +836,7 @@ int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_rows_kernel<T, BN>, a, w, x, split, x_tiles);
+  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_rows_kernel<T, BN>, a, w, x, split);
 }
 
 // Boxes of 32 rows by 128 bytes of y, for the stores; false where TMA cannot write.

@@ -624,10 +624,11 @@ def _layout(t):
 
 
 class _Described:
-    """Operators whose checks and descriptors are kept from call to call, by the layout of the inputs."""
+    """Operators whose checks and descriptors are kept from call to call, by the operator's settings and
+    the layout of the inputs."""
 
     def _described(self, handle, make, *tensors):
-        key = (handle.device, *map(_layout, tensors))
+        key = (handle.device, self._settings(), *map(_layout, tensors))
         kept = self.__dict__.setdefault("_kept", {})
         got = kept.get(key)
         if got is None:
@@ -656,6 +657,9 @@ class RMSNormalization(_Described, Operator):
     def from_node(cls, node, **kw):
         a = _attrs(node)
         return cls(a.get("epsilon", 1e-5), a.get("axis", -1), **kw)
+
+    def _settings(self):
+        return self.epsilon, self.axis, self.quantize
 
     def _check_axis(self, rank):
         if self.axis not in (-1, rank - 1):
@@ -720,6 +724,9 @@ class QuantizeBlocks(_Described, Operator):
             raise ValidationError(C.ERR_VALIDATION, f"QuantizeBlocks: block_rows must be 1 or {_QBLOCK}, got {block_rows}")
         self.block_rows = int(block_rows)
 
+    def _settings(self):
+        return self.block_rows
+
     @classmethod
     def from_node(cls, node, **kw):
         return cls(_attrs(node).get("block_rows", 1), **kw)
@@ -774,6 +781,9 @@ class MatMulBlockScaled(_Described, Operator):
                                   f"MatMulBlockScaled: expected float32, float16 or bfloat16, got {dtype}")
         self.dtype = dtype
         self.relu = bool(relu)
+
+    def _settings(self):
+        return self.dtype, self.relu
 
     @classmethod
     def from_node(cls, node, **kw):

@@ -422,6 +422,17 @@ def test_matmul_strides_and_bounds(handle, m, n, t):
             assert (rest == 3.0).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n", [(1, 517), (2, 129), (30, 517), (45, 130), (300, 517), (260, 1)])
+def test_matmul_ragged_columns_on_the_grid(handle, m, n, t):
+    """Output rows on the 16-byte grid whose last vector is cut: the columns behind it stay as they were."""
+    a, sa, b, sb = operands(m, n, 272, 6)
+    y = torch.full((m + 1, 544), 3.0, dtype=t, device="cuda")
+    run_mm(handle, a, sa, b, sb, None, y[:m, :n])
+    check_mm(y[:m, :n], a, sa, b, sb, None, False, t)
+    assert (y[:m, n:] == 3.0).all() and (y[m] == 3.0).all()
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 77, 333), (9, 128, 200), (130, 70, 257)])
 def test_matmul_unaligned_operands(ob, ctx, m, n, k):
     """Row strides and pointers that are no multiples of 16."""
@@ -564,6 +575,87 @@ def test_results_do_not_depend_on_the_run(ob, ctx):
         first = ob.MatMulBlockScaled().compute([a, sa, b, sb], ctx)[0]
         for _ in range(5):
             assert torch.equal(ob.MatMulBlockScaled().compute([a, sa, b, sb], ctx)[0], first)
+
+
+def test_settings_changed_between_calls(ob, ctx):
+    """Descriptors are kept by layout, but not past a change of the operator's own settings."""
+    x, w = normal((4, 256), 1), normal((256,), 2)
+    op = ob.RMSNormalization()
+    op.compute([x, w], ctx)
+    op.epsilon, op.quantize = 0.5, True
+    out = op.compute([x, w], ctx)
+    check_norm(out, x, None, w, 0.5, True)
+    a, sa, b, sb = operands(4, 8, 256, 1)
+    mm = ob.MatMulBlockScaled()
+    mm.compute([a, sa, b, sb], ctx)
+    mm.relu, mm.dtype = True, torch.float16
+    check_mm(mm.compute([a, sa, b, sb], ctx)[0], a, sa, b, sb, None, True, torch.float16)
+    q = ob.QuantizeBlocks()
+    q.compute([x], ctx)
+    q.block_rows = 128
+    assert q.compute([x], ctx)[1].shape == (1, 2)
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """A capture may be the first thing a process does with each kernel."""
+    import subprocess
+    import sys
+    code = """
+import importlib, torch
+ob = importlib.import_module("onnx-rs_b200")
+ctx = ob.ExecutionContext(ob.Handle(0))
+ins = [torch.randn(m, 512, device="cuda").bfloat16() for m in (1, 8, 100, 600)]
+w, wt = torch.ones(512, device="cuda").bfloat16(), torch.randn(384, 512, device="cuda")
+torch.cuda.synchronize()
+def run():
+    b, sb = ob.QuantizeBlocks(128).compute([wt], ctx)
+    out = []
+    for x in ins:
+        q, s = ob.RMSNormalization(quantize=True).compute([x, w], ctx)
+        out.append(ob.MatMulBlockScaled().compute([q, s, b, sb], ctx)[0])
+    return out
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+torch.cuda.synchronize()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) and torch.isfinite(x).all() for x, y in zip(got, want))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_two_handles_on_two_threads(ob):
+    """Each thread with a handle and a stream of its own, different sizes at the same time."""
+    import threading
+    jobs, errors = [], []
+    for i, (rows, cols) in enumerate(((3, 40001), (3, 13001))):
+        jobs.append((normal((rows, cols), i), normal((cols,), 7 + i), operands(20 + 300 * i, 640, 1024, i)))
+    torch.cuda.synchronize()
+
+    def work(x, w, mm):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                with ob.Handle(0) as h:
+                    ctx = ob.ExecutionContext(h)
+                    for _ in range(20):
+                        out = ob.RMSNormalization().compute([x, w], ctx)
+                        y = ob.MatMulBlockScaled().compute(list(mm), ctx)[0]
+                    h.synchronize()
+                    check_norm(out, x, None, w, 1e-5, False)
+                    check_mm(y, *mm, None, False, torch.float32)
+        except Exception as e:  # noqa: BLE001 -- handed to the test's thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    if errors:
+        raise errors[0]
 
 
 def test_current_device_is_kept(ob, ctx):
