@@ -34,6 +34,9 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(a, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(a, r); }
+
 // ---------------------------------------------------------------- CUDA cores
 // Operands that TMA cannot read (row strides or pointers off the 16-byte grid):
 // 64 x 64 outputs per block, 4 x 4 per thread; the products of a block of 128
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(kVecWarps * 32) matmul_blocks_vec_kernel(const
 }
 
 // ---------------------------------------------------------------- few rows
-// Three to 32 rows of a.  They are the MMA's N and the weights its M: a tile is 128
+// Three to 64 rows of a.  They are the MMA's N and the weights its M: a tile is 128
 // rows of b by all rows of a (BN >= m), so a handful of tokens wastes no tensor-core
 // rows and y's columns (n) lie along the lanes, whose stores are then contiguous.
 // The k range is split over the CTAs of a cluster; each leaves its partial sums in
@@ -465,11 +468,12 @@ struct PairLayout {
   static constexpr int kCW = BN * 4 / kPairEpiWarps;   // columns per epilogue warp
 };
 
-template <typename T, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+template <typename T, int BN, bool SPLIT>
+__global__ void __launch_bounds__(kPairThreads, 1)
     matmul_blocks_pair_kernel(const __grid_constant__ MatmulBlocksArgs p, const __grid_constant__ CUtensorMap tm_a,
                               const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_y,
-                              int tma_out) {
+                              int tma_out, int split) {
+  static_assert(!SPLIT || BN == 128, "the partial sums of a half would overwrite operands of the other's MMAs");
   using L = PairLayout<BN>;
   constexpr int ST = L::kStages, CW = L::kCW, NH = L::kHalves, NB = L::kBufs;
   extern __shared__ uint8_t smem_raw[];
@@ -488,7 +492,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  // rank in the pair, the pair's leader, and its slice of k (SPLIT: the pairs of a
+  // cluster share a tile)
+  const uint32_t crank = cluster_ctarank(), rank = SPLIT ? crank & 1 : crank, lead = SPLIT ? crank & ~1u : 0;
+  const uint16_t both = (uint16_t)(3u << lead);
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(full(s), 1);
@@ -520,8 +527,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   pdl_begin();
 
   const int tm = (p.m + 255) / 256, tn = (p.n + BN - 1) / BN;
-  const int tiles = tm * tn, pairs = gridDim.x / 2;
-  const int nkb = (p.k + kQBlock - 1) / kQBlock;
+  const int tiles = tm * tn, per_tile = SPLIT ? 2 * split : 2, pairs = gridDim.x / per_tile, tile0 = blockIdx.x / per_tile;
+  const int kbs = (p.k + kQBlock - 1) / kQBlock;
+  const int kb0 = SPLIT ? (int)((int64_t)kbs * (crank >> 1) / split) : 0;
+  const int nkb = SPLIT ? (int)((int64_t)kbs * ((crank >> 1) + 1) / split) - kb0 : kbs;
   auto tile_at = [&](int t, int& mt, int& nt) {
     const int per = kGroupM * tn, g = t / per, rem = t - g * per;
     const int rows = min(kGroupM, tm - g * kGroupM);
@@ -534,10 +543,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     constexpr int GPH = kPairEpiWarps / 4 / NH;  // groups of four warps per half
     const int sub = warp & 3, half = (warp >> 2) / GPH, within = (warp >> 2) % GPH * CW;
     const uint32_t lane_addr = tmem + ((uint32_t)(sub * 32) << 16) + half * 128 + within;
-    const uint32_t remote_empty = map_to_rank(acc_empty(half), 0);
+    const uint32_t remote_empty = map_to_rank(acc_empty(half), lead);
     const uint32_t sc = base + L::kOffScale + (half * 128 + sub * 32 + lane) * 16;
     uint32_t it = 0, group = 0;
-    for (int t = blockIdx.x / 2; t < tiles; t += pairs) {
+    for (int t = tile0; t < tiles; t += pairs) {
       uint64_t acc[CW / 2];
 #pragma unroll
       for (int j = 0; j < CW / 2; ++j) acc[j] = 0;
@@ -555,14 +564,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tc_fence_after();
           const uint64_t s2 = pack_f2(s, s);
           const uint32_t src = lane_addr + buf * (NH * 128);
-          // 16 columns are in flight while the 16 before them are added
-          uint32_t r[2][16];
-          tmem_ld_32x32b_x16(src, r[0]);
+          // LW columns are in flight while the LW before them are added (32 where the
+          // totals leave registers for it)
+          constexpr int LW = CW == 64 ? 32 : 16;
+          uint32_t r[2][LW];
+          tmem_ld(src, r[0]);
 #pragma unroll
-          for (int g = 0; g < CW / 16; ++g) {
+          for (int g = 0; g < CW / LW; ++g) {
             tmem_ld_wait();
-            if (g + 1 < CW / 16) {
-              tmem_ld_32x32b_x16(src + (g + 1) * 16, r[(g + 1) & 1]);
+            if (g + 1 < CW / LW) {
+              tmem_ld(src + (g + 1) * LW, r[(g + 1) & 1]);
             } else {
               tc_fence_before();
               __syncwarp();
@@ -570,13 +581,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             const uint32_t* q = r[g & 1];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              acc[g * 8 + j] =
-                  fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2, acc[g * 8 + j]);
+            for (int j = 0; j < LW / 2; ++j)
+              acc[g * (LW / 2) + j] = fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2,
+                                             acc[g * (LW / 2) + j]);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(sc_empty(g1));
+      }
+      if constexpr (SPLIT) {
+        // partial[column][row] in the stages: the last block's sums are here, so every
+        // MMA has run and every copy has landed
+        float* part = reinterpret_cast<float*>(gbase) + within * 128 + sub * 32 + lane;
+#pragma unroll
+        for (int j = 0; j < CW / 2; ++j) {
+          const float2 f = unpack_f2(acc[j]);
+          part[(2 * j) * 128] = f.x;
+          part[(2 * j + 1) * 128] = f.y;
+        }
+        break;
       }
       // Bias, Relu, rounding; then a warp's 32 rows go through its own staging
       // rows (swizzled as the TMA map wants them, which is also free of bank
@@ -673,7 +696,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+      for (int t = tile0; t < tiles && ok; t += pairs) {
         int mt, nt;
         tile_at(t, mt, nt);
         const int ra = mt * 256 + (int)rank * 128, rb = nt * BN + (int)rank * 64;
@@ -681,13 +704,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const int s = it % ST;
           ok = mbar_wait(empty(s), ((it / ST) & 1) ^ 1, abort_flag, p.status);
           if (!ok) break;
-          const uint32_t bar = map_to_rank(full(s), 0);
+          const uint32_t bar = map_to_rank(full(s), lead);
           if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * L::kStage);
           const uint32_t dst = base + s * L::kStage;
-          tma_load_2d_pair(dst, &tm_a, kb * kQBlock, ra, bar);
+          tma_load_2d_pair(dst, &tm_a, (kb0 + kb) * kQBlock, ra, bar);
 #pragma unroll
           for (int hf = 0; hf < NH; ++hf)  // this CTA's 64 rows of each half
-            tma_load_2d_pair(dst + L::kA + hf * 8192, &tm_b, kb * kQBlock, rb + hf * 128, bar);
+            tma_load_2d_pair(dst + L::kA + hf * 8192, &tm_b, (kb0 + kb) * kQBlock, rb + hf * 128, bar);
         }
       }
       // every copy has landed before the CTA may exit: the MMA of its stage has
@@ -703,7 +726,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const uint64_t da0 = smem_desc_sw128(base);  // a descriptor's address counts 16-byte units
       int s = 0, buf = 0;
       uint32_t sp = 0, bp = 1;  // parities: of the stage's use, of the buffer's release
-      const int total = nkb * ((tiles - (int)(blockIdx.x / 2) + pairs - 1) / pairs);
+      const int total = nkb * ((tiles - tile0 + pairs - 1) / pairs);
       for (int it = 0; it < total; ++it) {
         const uint64_t da = da0 + (uint64_t)(s * (L::kStage >> 4)), db = da + (L::kA >> 4);
         bar_wait(full(s), sp, abort_flag, p.status);
@@ -716,8 +739,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int kk = 0; kk < 4; ++kk)
               tc_mma_e4m3<2>(tmem + (buf * NH + hf) * 128, da + (uint64_t)(kk * 2), db + (uint64_t)(hf * 512 + kk * 2),
                              idesc, kk ? 1u : 0u);
-            if (hf == NH - 1) tc_commit_pair(empty(s));
-            tc_commit_pair(acc_full(buf * NH + hf));
+            if (hf == NH - 1) tc_commit_pair(empty(s), both);
+            tc_commit_pair(acc_full(buf * NH + hf), both);
           }
         }
         if (++s == ST) {
@@ -731,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       // every MMA has completed before TMEM is freed
       if (leader) {
-        tc_commit_pair(drain);
+        tc_commit_pair(drain, both);
         volatile int no_abort = 0;
         mbar_wait(drain, 0, &no_abort, p.status);
       }
@@ -742,7 +765,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // ahead: loaded before the buffer is waited for
     uint32_t group = 0;
     bool ok = true;
-    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+    for (int t = tile0; t < tiles && ok; t += pairs) {
       int mt, nt;
       tile_at(t, mt, nt);
       const int row = mt * 256 + (int)rank * 128 + lane;
@@ -750,7 +773,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         float va[4][4], vb[4][NH];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int k = min(kb + i, nkb - 1);
+          const int k = kb0 + min(kb + i, nkb - 1);
 #pragma unroll
           for (int j = 0; j < 4; ++j) va[i][j] = p.as[(int64_t)min(row + j * 32, p.m - 1) * p.as_row + k * p.as_block];
 #pragma unroll
@@ -771,10 +794,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // the pair's MMAs read both CTAs' shared memory and write both TMEMs
+  cluster_sync();  // the pair's MMAs read both CTAs' shared memory and write both TMEMs; partial sums
   if (warp == kPairEpiWarps + 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);
+  }
+  if constexpr (SPLIT) {
+    // Each pair finishes its share of the tile's columns, 8 at a time per thread (row):
+    // the slices' sums over distributed shared memory, in order.
+    if (warp < kPairEpiWarps) {
+      int mt, nt;
+      tile_at(tile0, mt, nt);
+      const int r = (warp & 3) * 32 + lane, row = mt * 256 + (int)rank * 128 + r;
+      const int share = BN / split, c0 = (int)(crank >> 1) * share + (warp >> 2) * (share / 2);
+      uint32_t from[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) from[q] = map_to_rank(base + r * 4, q < split ? 2 * q + rank : crank);
+      constexpr int PER = 16 / sizeof(T);
+      const bool vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.ldy % PER == 0;
+      for (int c = c0; c < c0 + share / 2; c += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float s[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) s[q] = ld_cluster_f32(from[q] + (c + j) * 512);
+          v[j] = s[0] + s[1];
+          if (split == 4) v[j] = v[j] + s[2] + s[3];
+        }
+        const int col = nt * BN + c;
+        if (row < p.m && col < p.n) {
+          T e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (p.bias) v[j] += p.bias[min(col + j, p.n - 1)];
+            if (p.relu) v[j] = v[j] < 0.f ? 0.f : v[j];  // NaN stays NaN
+            e[j] = from_f32<T>(v[j]);
+          }
+          T* dst = static_cast<T*>(p.y) + row * p.ldy + col;
+          if (vec && col + 8 <= p.n) {
+#pragma unroll
+            for (int u = 0; u < 8 / PER; ++u) reinterpret_cast<uint4*>(dst)[u] = reinterpret_cast<const uint4*>(e)[u];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (col + j < p.n) dst[j] = e[j];
+          }
+        }
+      }
+    }
+    cluster_sync_relaxed();  // no CTA leaves while another reads its partial sums
   }
 }
 
@@ -851,27 +920,31 @@ bool encode_out(const MatmulBlocksArgs& a, CUtensorMap* map) {
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int BN>
-int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st) {
+// split: pairs that share a tile (1, 2 or 4; BN == 128).
+template <typename T, int BN, bool SPLIT = false>
+int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st, int split = 1) {
   using L = PairLayout<BN>;
   CUtensorMap ma, mb, my{};
   if (!encode_rows(a.a, a.m, a.k, a.lda, 128, &ma) || !encode_rows(a.b, a.n, a.k, a.ldb, 64, &mb))
     return (int)cudaErrorInvalidValue;
-  const int tma_out = encode_out<T>(a, &my);
-  int rc = opt_in<matmul_blocks_pair_kernel<T, BN>>(L::kBytes);
+  const int tma_out = SPLIT ? 0 : encode_out<T>(a, &my);
+  int rc = opt_in<matmul_blocks_pair_kernel<T, BN, SPLIT>>(L::kBytes);
   if (rc) return rc;
   const int tiles = ((a.m + 255) / 256) * ((a.n + BN - 1) / BN);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2u * std::min(tiles, num_sms / 2));
+  cfg.gridDim = dim3(2u * split * (SPLIT ? tiles : std::min(tiles, num_sms / 2)));
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2u * split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN>, a, ma, mb, my, tma_out);
+  cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN, SPLIT>, a, ma, mb, my, tma_out, split);
 }
 
 }  // namespace
@@ -885,12 +958,21 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       return launch_pdl(matmul_blocks_simt_kernel<T>, (unsigned)((a.n + 63) / 64) * ((a.m + 63) / 64), 256, 0, st, a);
     }
     const int kbs = (a.k + kQBlock - 1) / kQBlock;
-    if (a.m > 32) {
+    // 33 to 64 rows with few columns stay with the kernel for few rows, whose clusters
+    // split k eight ways (64 x 4096 x 4096: 10.7 us, 12.5 on pairs; with 64 tiles of
+    // columns, 64 x 8192 x 4096, 18.7 and 15.4).
+    if (a.m > 64 || (a.m > 32 && (a.n + 127) / 128 * 4 > num_sms)) {
       // Tiles of 256 x 256 or 256 x 128 on num_sms / 2 pairs: a wave of the narrow
       // ones takes ~0.6 of a wave of the wide ones (8.5 and 16 us at k = 4096; 200 x
       // 8192: 15.3 and 20.4 us, 512 x 8192: 23.4 and 21.4 us, 4096 x 4096: 70.6 and 67.2 us).
       const int64_t tm = (a.m + 255) / 256, pairs = num_sms / 2;
       const int64_t wide = (tm * ((a.n + 255) / 256) + pairs - 1) / pairs, narrow = (tm * ((a.n + 127) / 128) + pairs - 1) / pairs;
+      // Few tiles: two or four pairs share one, each a slice of k of four blocks at
+      // least (128 x 4096 x 14336: 23.2 us with two, 36 with one; 256 x 4096 x 4096: 13.3
+      // and 14.5).
+      const int64_t tiles = tm * ((a.n + 127) / 128);
+      if (tiles * 4 <= pairs && kbs >= 16) return launch_pair<T, 128, true>(a, num_sms, st, 4);
+      if (tiles * 2 <= pairs && kbs >= 8) return launch_pair<T, 128, true>(a, num_sms, st, 2);
       return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
     }
     const size_t vec_smem = (size_t)a.m * ((a.k + 15) / 16 * 32 + kbs * 4);
@@ -903,7 +985,9 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
     const int tiles = (a.n + 127) / 128;
     int split = tiles * 4 <= num_sms * 3 && kbs >= 4 ? 2 : 1;
     while (split > 1 && split < 8 && tiles * split <= num_sms && kbs >= split * 4) split *= 2;
-    return a.m <= 16 ? launch_rows<T, 16>(a, split, st) : launch_rows<T, 32>(a, split, st);
+    return a.m <= 16   ? launch_rows<T, 16>(a, split, st)
+           : a.m <= 32 ? launch_rows<T, 32>(a, split, st)
+                       : launch_rows<T, 64>(a, split, st);
   });
 }
 

@@ -434,12 +434,12 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(cluster_bar)
       : "memory");
 }
-// Arrive on the barrier at `bar`'s offset in both CTAs of the pair once every MMA issued so
-// far by this thread has completed.
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+// Arrive on the barrier at `bar`'s offset in the CTAs of `mask` (the pair's two ranks in
+// the cluster) once every MMA issued so far by this thread has completed.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"((uint16_t)3)
+      "h"(mask)
       : "memory");
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
