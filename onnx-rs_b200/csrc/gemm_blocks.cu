@@ -246,7 +246,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc + 4);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (a shuffle tells the compiler that it is the same in all lanes: TMEM addresses and
+  // barriers then stay in uniform registers)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(full(s), 1);
@@ -491,7 +493,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kOffMisc + 4);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (a shuffle tells the compiler that it is the same in all lanes: TMEM addresses and
+  // barriers then stay in uniform registers)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // rank in the pair, the pair's leader, and its slice of k (SPLIT: the pairs of a
   // cluster share a tile)
   const uint32_t crank = cluster_ctarank(), rank = SPLIT ? crank & 1 : crank, lead = SPLIT ? crank & ~1u : 0;
