@@ -134,22 +134,24 @@ __device__ __forceinline__ bool writes_scale() {
   return (threadIdx.x & (16 / N - 1)) == 0;
 }
 
-// Rows whose every vector is aligned: one row per block, CH vectors of eight
-// columns per thread, read once and kept in registers; the weight is on its way
+// Rows whose every vector is aligned: one row per block, or (WARP) per warp of a block
+// of 256 threads, CH vectors of eight columns per thread, read once and kept in
+// registers; the weight is on its way
 // before the row's one reduction (a shuffle and a barrier).  Bound by HBM with
 // several blocks per SM taking turns; blocks that walk rows with the next two rows
 // copied ahead were slower (107 against 84 us then: fewer blocks, and the same chain
 // of reductions).  8192 x 8192 bf16 with residual and e4m3 output (470 MB): 74 us,
 // 6.3 TB/s; one row of 4096 2.8 us.
-template <typename T, typename W, int CH>
-__global__ void __launch_bounds__(CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 2 ? 2 : 1)
+template <typename T, typename W, int CH, bool WARP = false>
+__global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 2 ? (WARP ? 4 : 2) : 1)
     rmsnorm_vec_kernel(const RmsNormArgs p) {
   __shared__ float part[32];
   pdl_begin();
-  const int64_t r = blockIdx.x;
-  const int n8 = p.cols / 8, nt = blockDim.x;
+  const int64_t r = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && r >= p.rows) return;
+  const int n8 = p.cols / 8, nt = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
   // vector c of this thread; threads past the row's end work on zeros
-  auto at = [&](int c) { return c * nt + (int)threadIdx.x; };
+  auto at = [&](int c) { return c * nt + tid; };
   const T* x = static_cast<const T*>(p.x) + r * p.ldx;
   float h[CH][8];
   {
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = fmaf(h[c][j], h[c][j], ss);
   ss = warp_sum(ss);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
+  if (!WARP && (threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
   if (p.sum) {
     T* sum = static_cast<T*>(p.sum) + r * p.lds;
 #pragma unroll
@@ -193,9 +195,11 @@ __global__ void __launch_bounds__(CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 
       if (at(c) < n8) o.store(sum + at(c) * 8);
     }
   }
-  __syncthreads();
-  ss = (threadIdx.x & 31) < nt / 32 ? part[threadIdx.x & 31] : 0.f;
-  ss = warp_sum(ss);
+  if (!WARP) {
+    __syncthreads();
+    ss = (threadIdx.x & 31) < nt / 32 ? part[threadIdx.x & 31] : 0.f;
+    ss = warp_sum(ss);
+  }
   const float rstd = 1.f / sqrtf(ss / (float)p.cols + p.eps);
   float amax[CH];
 #pragma unroll
@@ -480,11 +484,19 @@ int rmsnorm_launch(const RmsNormArgs& a, int num_sms, cudaStream_t st) {
         }
         return launch_pdl(rmsnorm_row_kernel<T, W>, (unsigned)a.rows, kRowThreads, smem, st, a);
       }
-      // vectors per thread: 256 threads a row when there are rows enough to fill the
-      // GPU (more loads in flight per thread, cheaper reductions), as many threads as
-      // there are vectors when there are not
+      // With rows enough to fill the GPU: a warp a row up to 1024 columns (8192 x 128
+      // bf16: 3.3 us against 10.0 with a block a row), then few threads with more
+      // loads in flight each and cheaper reductions (8192 x 2048: 20.9 us with 128
+      // threads, 23.2 with 256).  Otherwise as many threads as there are vectors.
       const int n8 = a.cols / 8;
-      const int want = a.rows <= 2 * num_sms ? 1024 : 256;
+      const bool many = a.rows > 2 * num_sms;
+      if (many && n8 <= 128) {
+        const unsigned grid = (unsigned)((a.rows + 7) / 8);
+        if (n8 <= 32) return launch_pdl(rmsnorm_vec_kernel<T, W, 1, true>, grid, 256, 0, st, a);
+        if (n8 <= 64) return launch_pdl(rmsnorm_vec_kernel<T, W, 2, true>, grid, 256, 0, st, a);
+        return launch_pdl(rmsnorm_vec_kernel<T, W, 4, true>, grid, 256, 0, st, a);
+      }
+      const int want = many ? 128 : 1024;
       const int ch = n8 <= want ? 1 : n8 <= 2 * want ? 2 : 4;
       const int threads = std::min(1024, ((n8 + ch - 1) / ch + 31) / 32 * 32);
       if (ch == 1) return launch_pdl(rmsnorm_vec_kernel<T, W, 1>, (unsigned)a.rows, threads, 0, st, a);
