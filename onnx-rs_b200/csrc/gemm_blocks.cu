@@ -463,11 +463,12 @@ struct PairLayout {
   static constexpr int kOffOut = kStages * kStage;
   static constexpr int kOffScale = kOffOut + kPairEpiWarps * kOutWarp;  // two groups: [halves][128] rows of four blocks
   static constexpr int kScaleGroup = 4 * kHalves * 128;
-  static constexpr int kOffBar = kOffScale + 2 * kScaleGroup * 4;
+  static constexpr int kCW = BN * 4 / kPairEpiWarps;   // columns per epilogue warp
+  static constexpr int kOffBias = kOffScale + 2 * kScaleGroup * 4;      // per epilogue warp: its columns' bias
+  static constexpr int kOffBar = kOffBias + kPairEpiWarps * kCW * 4;
   static constexpr int kBars = 2 * kStages + 13;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kBytes = kOffMisc + 16 + 1024;
-  static constexpr int kCW = BN * 4 / kPairEpiWarps;   // columns per epilogue warp
 };
 
 template <typename T, int BN, bool SPLIT>
@@ -551,6 +552,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t sc = base + L::kOffScale + (half * 128 + sub * 32 + lane) * 16;
     uint32_t it = 0, group = 0;
     for (int t = tile0; t < tiles; t += pairs) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
+      const int col0 = nt * BN + half * 128 + within;
+      if (!SPLIT && p.bias) {  // here, where the first block is waited for anyway
+        float* bias = reinterpret_cast<float*>(gbase + L::kOffBias) + warp * CW;
+#pragma unroll
+        for (int j = 0; j < CW; j += 32) bias[j + lane] = col0 + j + lane < p.n ? p.bias[col0 + j + lane] : 0.f;
+      }
       uint64_t acc[CW / 2];
 #pragma unroll
       for (int j = 0; j < CW / 2; ++j) acc[j] = 0;
@@ -609,10 +619,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // rows (swizzled as the TMA map wants them, which is also free of bank
       // conflicts) to TMA stores that clip the tile's edges; where TMA cannot
       // write (y, or its last column, off the 16-byte grid), element by element.
-      int mt, nt;
-      tile_at(t, mt, nt);
-      const int row0 = mt * 256 + (int)rank * 128 + sub * 32;
-      const int col0 = nt * BN + half * 128 + within;
       constexpr int ES = sizeof(T), PER = 16 / ES, CPR = 128 / ES;  // columns of a 16-byte unit, of a staging row
       constexpr int NC = CW / CPR, OB = NC < L::kOutBufs ? NC : L::kOutBufs;
       const uint32_t out = base + L::kOffOut + warp * L::kOutWarp;
@@ -634,12 +640,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 f[q + 1] = v.y;
               }
               if constexpr (decltype(extras)::value) {
-                const int j0 = col0 + c * CPR + u * PER;
+                if (p.bias) {
+                  const float4* b4 = reinterpret_cast<const float4*>(gbase + L::kOffBias) + (warp * CW + c * CPR + u * PER) / 4;
 #pragma unroll
-                for (int q = 0; q < PER; ++q) {
-                  if (p.bias) f[q] += p.bias[min(j0 + q, p.n - 1)];
-                  if (p.relu) f[q] = f[q] < 0.f ? 0.f : f[q];  // NaN stays NaN
+                  for (int q = 0; q < PER; q += 4) {
+                    const float4 b = b4[q / 4];
+                    f[q] += b.x;
+                    f[q + 1] += b.y;
+                    f[q + 2] += b.z;
+                    f[q + 3] += b.w;
+                  }
                 }
+#pragma unroll
+                for (int q = 0; q < PER; ++q)
+                  if (p.relu) f[q] = f[q] < 0.f ? 0.f : f[q];  // NaN stays NaN
               }
               uint32_t w[4];
 #pragma unroll
