@@ -578,8 +578,16 @@ def _stored_scales(lead, rows, blocks):
     return (*lead, blocks), (*strides, max(1, rows)), torch.float32
 
 
-def _new(spec, dev):
-    return torch.empty_strided(spec[0], spec[1], dtype=spec[2], device=dev)
+# torch.empty_strided on the current device without its keyword arguments' parsing: 0.8 instead of
+# 1.5 us of a call of 9 to 12.  It is not a public name, so it may be missing.
+_new_here = getattr(getattr(torch._C._dynamo, "guards", None), "_empty_strided_cuda", None)
+
+
+def _new_on(dev):
+    """f(shape, strides, dtype): a new uninitialised tensor on a device."""
+    if _new_here is not None and dev.type == "cuda" and dev.index == torch._C._cuda_getDevice():
+        return _new_here
+    return lambda shape, strides, dtype: torch.empty_strided(shape, strides, dtype=dtype, device=dev)
 
 
 def _scale_strides(s, rows, blocks, what):
@@ -703,10 +711,10 @@ class RMSNormalization(_Described, Operator):
         x, w = inputs[0], inputs[1]
         h = ctx.handle
         _, desc, y_spec, qs_spec, sum_spec = self._described(h, self._describe, x, w, residual)
-        dev = x.device
-        y = _new(y_spec, dev)
-        qs = _new(qs_spec, dev) if qs_spec else None
-        total = _new(sum_spec, dev) if sum_spec else None
+        new = _new_on(x.device)
+        y = new(*y_spec)
+        qs = new(*qs_spec) if qs_spec else None
+        total = new(*sum_spec) if sum_spec else None
         _launch(h, "RMSNormalization", C.lib().onnxb200_rmsnorm, desc, x.data_ptr(), _ptr(residual), w.data_ptr(),
                 _ptr(total), y.data_ptr(), _ptr(qs))
         out = [y] if qs is None else [y, qs]
@@ -762,7 +770,8 @@ class QuantizeBlocks(_Described, Operator):
         x = inputs[0]
         h = ctx.handle
         _, desc, q_spec, s_spec = self._described(h, self._describe, x)
-        q, s = _new(q_spec, x.device), _new(s_spec, x.device)
+        new = _new_on(x.device)
+        q, s = new(*q_spec), new(*s_spec)
         _launch(h, "QuantizeBlocks", C.lib().onnxb200_quantize_blocks, desc, x.data_ptr(), q.data_ptr(), s.data_ptr())
         return [q, s]
 
@@ -831,7 +840,7 @@ class MatMulBlockScaled(_Described, Operator):
             a_scale = _scale_strides(a_scale, copy_a, blocks, self.op_type)[0]
         if copy_b is not None:
             b_scale = _scale_strides(b_scale, copy_b, blocks, self.op_type)[0]
-        y = _new(y_spec, a.device)
+        y = _new_on(a.device)(*y_spec)
         _launch(h, "MatMulBlockScaled", C.lib().onnxb200_matmul_blocks, desc, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
                 b_scale.data_ptr(), _ptr(bias), y.data_ptr())
         return [y]

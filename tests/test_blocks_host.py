@@ -134,7 +134,7 @@ def test_row_stride(ob):
 
 
 def test_stored_layouts(ob):
-    new = lambda spec: ob.ops._new(spec, "cpu")
+    new = lambda spec: ob.ops._new_on(torch.device("cpu"))(*spec)
     q = new(ob.ops._stored_rows((3, 2), 33))
     assert q.shape == (3, 2, 33) and ob.ops._stored_stride(33) == 48 and ob.ops._row_stride(q, "q") == 48
     q = new(ob.ops._stored_rows((), 64))

@@ -333,7 +333,8 @@ def check_mm(y, a, sa, b, sb, bias, relu, t):
 
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (1, 1000, 2048), (2, 300, 1000), (8, 8, 16), (15, 129, 127), (16, 256, 128),
           (17, 1000, 2048), (33, 100, 640), (64, 130, 4096), (65, 512, 256), (127, 257, 300), (128, 128, 1024), (129, 640, 48),
-          (200, 2048, 512), (256, 256, 256), (257, 511, 129), (500, 1000, 1100), (1024, 512, 768), (777, 1300, 400), (2049, 300, 200)]
+          (200, 2048, 512), (256, 256, 256), (257, 511, 129), (500, 1000, 1100), (1024, 512, 768), (777, 1300, 400), (2049, 300, 200),
+          (1, 64, 60000), (2, 130, 30000), (3, 70, 20011), (40, 200, 12345), (65, 300, 2200), (100, 140, 9999), (300, 260, 7777)]
 
 
 @pytest.mark.parametrize("t", TYPES)
