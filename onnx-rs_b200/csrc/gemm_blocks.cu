@@ -34,8 +34,6 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(a, r); }
-__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(a, r); }
 
 // ---------------------------------------------------------------- CUDA cores
 // Operands that TMA cannot read (row strides or pointers off the 16-byte grid):
@@ -435,15 +433,19 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 // walk the tiles, and a tile's stores (TMA, from shared memory) run under the
 // next tile's loads and MMAs.
 //
-// What bounds it: at 256 x 256 a block of 128 k's takes 730 cycles, of which the
+// What bounds it: at 256 x 256 a block of 128 k's takes 710 cycles, of which the
 // MMAs need 512 (a pure stream of them measured 512, at 1.4 GHz under the power cap
-// 3.3 PFLOP/s); the rest is the round trip MMA -> commit -> 8 reads of 16 TMEM
-// columns -> arrival on the leader, which two accumulators per half do not cover.
-// TMEM is full, and so are the registers: reads of 32 columns, or sixteen warps with
-// half the totals each, spilled and were slower (8192^3: 568 and 580 us against 490),
-// as were both halves in every warp (525) and asking barriers one block ahead (498).
-// 8192^3 bf16: 465-500 us, 2.2-2.4 PFLOP/s; 4096^3 62 us; 8192 x 8192 x 1024 74 us;
-// 200 x 8192 x 4096 (256 x 128 tiles, 36 MB) 15 us, its loop at 4.7 TB/s.
+// 3.3 PFLOP/s).  With a quarter of the columns read and added it took 620, with half
+// of the operands loaded as well 600: the rest is the round trip MMA -> commit ->
+// reads -> arrival on the leader, which two accumulators per half do not cover, and
+// the clock, 1.2 to 1.4 GHz at the power cap.  TMEM is full, and so are the registers:
+// with sixteen columns in flight instead of 64 8192^3 took 523 instead of 503 us,
+// with the next block's first columns loaded under the last additions 600 (register
+// moves), with sixteen warps and half the totals each 580 (spills).
+// Run without a pause (1.24 to 1.5 GHz): 8192^3 bf16 508 us, 2.16 PFLOP/s; 4096^3 72
+// us; 8192 x 8192 x 1024 80 us (its tiles' output is a sixth); after idle, at higher
+// clocks, 8192^3 435 us.  200 x 8192 x 4096 (256 x 128 tiles, 36 MB) 15 us, its loop
+// at 4.7 TB/s.
 //
 // 8 epilogue warps, then a warpgroup with the TMA, MMA and scale warps.  Launched
 // with 168 registers a thread (384 x 168 = 64512), split as 208 for the totals and
@@ -578,27 +580,32 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tc_fence_after();
           const uint64_t s2 = pack_f2(s, s);
           const uint32_t src = lane_addr + buf * (NH * 128);
-          // LW columns are in flight while the LW before them are added (32 where the
-          // totals leave registers for it)
-          constexpr int LW = CW == 64 ? 32 : 16;
-          uint32_t r[2][LW];
-          tmem_ld(src, r[0]);
+          // 64 columns arrive per wait (the wait is for every load before it); of 128,
+          // each 16 of the second half are loaded into the registers of the 16 just added
+          uint32_t r[4][16];
+          auto add = [&](int g) {
+            const uint32_t* q = r[g % 4];
 #pragma unroll
-          for (int g = 0; g < CW / LW; ++g) {
-            tmem_ld_wait();
-            if (g + 1 < CW / LW) {
-              tmem_ld(src + (g + 1) * LW, r[(g + 1) & 1]);
-            } else {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_remote(remote_empty + buf * (NH * 8));
+            for (int j = 0; j < 8; ++j)
+              acc[g * 8 + j] =
+                  fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2, acc[g * 8 + j]);
+          };
+#pragma unroll
+          for (int g = 0; g < 4; ++g) tmem_ld_32x32b_x16(src + g * 16, r[g]);
+          tmem_ld_wait();
+          if constexpr (CW == 128) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              add(g);
+              tmem_ld_32x32b_x16(src + 64 + g * 16, r[g]);
             }
-            const uint32_t* q = r[g & 1];
-#pragma unroll
-            for (int j = 0; j < LW / 2; ++j)
-              acc[g * (LW / 2) + j] = fma_f2(pack_f2(__uint_as_float(q[2 * j]), __uint_as_float(q[2 * j + 1])), s2,
-                                             acc[g * (LW / 2) + j]);
+            tmem_ld_wait();
           }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(remote_empty + buf * (NH * 8));
+#pragma unroll
+          for (int g = CW / 16 - 4; g < CW / 16; ++g) add(g);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(sc_empty(g1));
