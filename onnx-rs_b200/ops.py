@@ -635,6 +635,9 @@ class _Described:
     """Operators whose checks and descriptors are kept from call to call, by the operator's settings and
     the layout of the inputs."""
 
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_kept"}  # pointers are neither copied nor pickled
+
     def _described(self, handle, make, *tensors):
         key = (handle.device, self._settings(), *map(_layout, tensors))
         kept = self.__dict__.setdefault("_kept", {})

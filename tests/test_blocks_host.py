@@ -201,3 +201,19 @@ def test_registry_and_shapes(ob):
         mm.validate({"inputs": ["a", "as", "b"], "outputs": ["y"]})
     with pytest.raises(ob.ValidationError):
         r.create_operator_for_node({**mn, "attrs": {"dtype": 7}})
+
+
+def test_operators_are_copied_and_pickled_after_a_call(ob):
+    """What a call keeps holds pointers to this process's descriptors: it stays out of copies."""
+    import copy
+    import pickle
+    import types
+
+    for op in (ob.RMSNormalization(1e-6, quantize=True), ob.QuantizeBlocks(128), ob.MatMulBlockScaled(torch.float16, True)):
+        op._described(types.SimpleNamespace(device=0), lambda h, x: (ctypes.byref(C_INT),), torch.zeros(3))
+        for other in (copy.copy(op), copy.deepcopy(op), pickle.loads(pickle.dumps(op))):
+            assert type(other) is type(op) and other._settings() == op._settings()
+            assert "_kept" in op.__dict__ and "_kept" not in other.__dict__
+
+
+C_INT = ctypes.c_int()
