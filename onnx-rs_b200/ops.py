@@ -17,12 +17,18 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
 from typing import Dict, List, Optional, Sequence
 
 import torch
 
 from . import _capi as C
 from .runtime import (Handle, InvalidOperator, UnsupportedFeature, ValidationError, dptr)
+
+# the native module for repeated calls (make -C csrc calls); ctypes does without it
+_calls = None
+if os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "_calls.so")):
+    from . import _calls
 
 
 class ExecutionContext:
@@ -578,15 +584,8 @@ def _stored_scales(lead, rows, blocks):
     return (*lead, blocks), (*strides, max(1, rows)), torch.float32
 
 
-# torch.empty_strided on the current device without its keyword arguments' parsing: 0.8 instead of
-# 1.5 us of a call of 9 to 12.  It is not a public name, so it may be missing.
-_new_here = getattr(getattr(torch._C._dynamo, "guards", None), "_empty_strided_cuda", None)
-
-
 def _new_on(dev):
     """f(shape, strides, dtype): a new uninitialised tensor on a device."""
-    if _new_here is not None and dev.type == "cuda" and dev.index == torch._C._cuda_getDevice():
-        return _new_here
     return lambda shape, strides, dtype: torch.empty_strided(shape, strides, dtype=dtype, device=dev)
 
 
@@ -622,6 +621,10 @@ def _launch(h, what, entry, desc, *args):
         h.check(rc, what)
 
 
+def _address(fn):
+    return ctypes.cast(fn, ctypes.c_void_p).value
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -632,11 +635,38 @@ def _layout(t):
 
 
 class _Described:
-    """Operators whose checks and descriptors are kept from call to call, by the operator's settings and
-    the layout of the inputs."""
+    """Operators whose checks, descriptors and output layouts are kept from call to call, by the
+    operator's settings and the layout of the inputs.  Where the native module _calls is built, a call
+    whose layouts were seen before is made there (csrc/torch_calls.cpp)."""
+    entry = None   # name of the C entry
+    slots = ()     # its pointers behind the descriptor: an input, or -1 - an output
+
+    def __setattr__(self, name, value):
+        """A changed setting: what was kept does not hold any more."""
+        object.__setattr__(self, name, value)
+        self.__dict__.pop("_kept", None)
+        self.__dict__.pop("_plans", None)
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k != "_kept"}  # pointers are neither copied nor pickled
+        # pointers are neither copied nor pickled
+        return {k: v for k, v in self.__dict__.items() if k not in ("_kept", "_plans")}
+
+    def _call(self, h, *tensors):
+        plans = self.__dict__.get("_plans")
+        if plans and h.ptr:
+            out = _calls.run(plans, h.ptr.value, h.device, h.own_stream_ptr, *tensors)
+            if out.__class__ is list:
+                return out
+            if out is not None:
+                h.check(out, self.op_type)
+        desc, specs, relaid = self._described(h, self._prepare, *tensors)
+        for i, lay in relaid:
+            tensors = (*tensors[:i], lay(tensors[i]), *tensors[i + 1:])
+        new = _new_on(tensors[0].device)
+        outs = [None if spec is None else new(*spec) for spec in specs]
+        _launch(h, self.op_type, getattr(C.lib(), self.entry), ctypes.byref(desc),
+                *(_ptr(tensors[s] if s >= 0 else outs[-1 - s]) for s in self.slots))
+        return [t for t in outs if t is not None]
 
     def _described(self, handle, make, *tensors):
         key = (handle.device, self._settings(), *map(_layout, tensors))
@@ -645,7 +675,21 @@ class _Described:
         if got is None:
             if len(kept) >= 64:
                 kept.clear()
+                self.__dict__.pop("_plans", None)
             got = kept[key] = make(handle, *tensors)
+        return got
+
+    def _prepare(self, h, *tensors):
+        """Checks a call and keeps it for _calls.run; the newest comes first."""
+        desc, specs, relaid = got = self._describe(h, *tensors)
+        if _calls is None or relaid:
+            return got
+        present = [i for i, spec in enumerate(specs) if spec is not None]
+        slots = tuple((s if tensors[s] is not None else None) if s >= 0 else
+                      (-1 - present.index(-1 - s) if specs[-1 - s] is not None else None) for s in self.slots)
+        plan = _calls.Plan(_address(getattr(C.lib(), self.entry)), _address(C.lib().onnxb200_get_stream),
+                           ctypes.addressof(desc), desc, h.device, tensors, tuple(specs[i] for i in present), slots)
+        self.__dict__.setdefault("_plans", []).insert(0, plan)
         return got
 
 
@@ -658,6 +702,8 @@ class RMSNormalization(_Described, Operator):
     type) is returned as the last output."""
     op_type = "RMSNormalization"
     min_inputs = 2
+    entry = "onnxb200_rmsnorm"
+    slots = (0, 2, 1, -3, -1, -2)  # x, residual, scale; h, y, y_scale
 
     def __init__(self, epsilon=1e-5, axis=-1, quantize=False):
         self.epsilon = float(epsilon)
@@ -707,21 +753,11 @@ class RMSNormalization(_Described, Operator):
             d.y_scale_row, d.y_scale_block = 1, max(1, rows)
         blocks = (cols + _QBLOCK - 1) // _QBLOCK
         same = _dense(x.shape, x.dtype)
-        return (d, ctypes.byref(d), _stored_rows(lead, cols) if self.quantize else same,
-                _stored_scales(lead, rows, blocks) if self.quantize else None, same if residual is not None else None)
+        return d, (_stored_rows(lead, cols) if self.quantize else same,
+                   _stored_scales(lead, rows, blocks) if self.quantize else None, same if residual is not None else None), ()
 
     def compute(self, inputs, ctx, residual=None):
-        x, w = inputs[0], inputs[1]
-        h = ctx.handle
-        _, desc, y_spec, qs_spec, sum_spec = self._described(h, self._describe, x, w, residual)
-        new = _new_on(x.device)
-        y = new(*y_spec)
-        qs = new(*qs_spec) if qs_spec else None
-        total = new(*sum_spec) if sum_spec else None
-        _launch(h, "RMSNormalization", C.lib().onnxb200_rmsnorm, desc, x.data_ptr(), _ptr(residual), w.data_ptr(),
-                _ptr(total), y.data_ptr(), _ptr(qs))
-        out = [y] if qs is None else [y, qs]
-        return out if total is None else out + [total]
+        return self._call(ctx.handle, inputs[0], inputs[1], residual)
 
 
 class QuantizeBlocks(_Described, Operator):
@@ -729,6 +765,8 @@ class QuantizeBlocks(_Described, Operator):
     gives one scale for every 128 columns of a row (activations, any leading dims), block_rows = 128
     one for 128 rows by 128 columns (weights, 2-D).  Not in the reference registry."""
     op_type = "QuantizeBlocks"
+    entry = "onnxb200_quantize_blocks"
+    slots = (0, -1, -2)
 
     def __init__(self, block_rows=1):
         if block_rows not in (1, _QBLOCK):
@@ -766,17 +804,11 @@ class QuantizeBlocks(_Described, Operator):
             d.scale_row, d.scale_block = 1, max(1, rows)
         else:
             d.scale_row, d.scale_block = max(1, blocks), 1
-        return (d, ctypes.byref(d), _stored_rows(lead, cols), _stored_scales(lead, rows, blocks) if self.block_rows == 1 else
-                _dense(((rows + _QBLOCK - 1) // _QBLOCK, blocks), torch.float32))
+        return d, (_stored_rows(lead, cols), _stored_scales(lead, rows, blocks) if self.block_rows == 1 else
+                   _dense(((rows + _QBLOCK - 1) // _QBLOCK, blocks), torch.float32)), ()
 
     def compute(self, inputs, ctx):
-        x = inputs[0]
-        h = ctx.handle
-        _, desc, q_spec, s_spec = self._described(h, self._describe, x)
-        new = _new_on(x.device)
-        q, s = new(*q_spec), new(*s_spec)
-        _launch(h, "QuantizeBlocks", C.lib().onnxb200_quantize_blocks, desc, x.data_ptr(), q.data_ptr(), s.data_ptr())
-        return [q, s]
+        return self._call(ctx.handle, inputs[0])
 
 
 class MatMulBlockScaled(_Described, Operator):
@@ -786,6 +818,8 @@ class MatMulBlockScaled(_Described, Operator):
     [..., n] in ``dtype``, after Relu if asked.  Not in the reference registry."""
     op_type = "MatMulBlockScaled"
     min_inputs = 4
+    entry = "onnxb200_matmul_blocks"
+    slots = (0, 1, 2, 3, 4, -1)
 
     def __init__(self, dtype=torch.float32, relu=False):
         if dtype not in _TYPE:
@@ -825,28 +859,19 @@ class MatMulBlockScaled(_Described, Operator):
             raise ValidationError(C.ERR_VALIDATION, f"{what}: expected a contiguous float32 bias of {n} elements")
         d.m, d.n, d.k = m, n, k
         # scales that are not addressable by two strides are laid out anew on every call
-        lay = []
-        for s, rows in ((a_scale, m), (b_scale, rows_b)):
+        strides, relaid = [], []
+        for i, s, rows in ((1, a_scale, m), (3, b_scale, rows_b)):
             t, sr, sb = _scale_strides(s, rows, blocks, what)
-            lay += [sr, sb, rows if t.data_ptr() != s.data_ptr() else None]
-        d.a_scale_row, d.a_scale_block, copy_a, d.b_scale_row, d.b_scale_block, copy_b = lay
+            strides += [sr, sb]
+            if t.data_ptr() != s.data_ptr():
+                relaid.append((i, lambda s, rows=rows: _scale_strides(s, rows, blocks, what)[0]))
+        d.a_scale_row, d.a_scale_block, d.b_scale_row, d.b_scale_block = strides
         d.out_type = _TYPE[self.dtype]
         d.flags = C.EPI_RELU if self.relu else 0
-        return d, ctypes.byref(d), _dense((*a.shape[:-1], n), self.dtype), copy_a, copy_b, blocks
+        return d, (_dense((*a.shape[:-1], n), self.dtype),), relaid
 
     def compute(self, inputs, ctx):
-        a, a_scale, b, b_scale = inputs[:4]
-        bias = inputs[4] if len(inputs) > 4 else None
-        h = ctx.handle
-        _, desc, y_spec, copy_a, copy_b, blocks = self._described(h, self._describe, a, a_scale, b, b_scale, bias)
-        if copy_a is not None:
-            a_scale = _scale_strides(a_scale, copy_a, blocks, self.op_type)[0]
-        if copy_b is not None:
-            b_scale = _scale_strides(b_scale, copy_b, blocks, self.op_type)[0]
-        y = _new_on(a.device)(*y_spec)
-        _launch(h, "MatMulBlockScaled", C.lib().onnxb200_matmul_blocks, desc, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(),
-                b_scale.data_ptr(), _ptr(bias), y.data_ptr())
-        return [y]
+        return self._call(ctx.handle, *inputs[:4], inputs[4] if len(inputs) > 4 else None)
 
 
 # --------------------------------------------------------------------------- registry

@@ -217,3 +217,31 @@ def test_operators_are_copied_and_pickled_after_a_call(ob):
 
 
 C_INT = ctypes.c_int()
+
+
+def test_module_for_repeated_calls(ob, C):
+    """Plans are checked when they are made, and fit nothing on the CPU."""
+    calls = ob.ops._calls
+    if calls is None:
+        pytest.skip("onnx-rs_b200/_calls.so is not built")
+    x, d = torch.zeros(2, 3), quant_desc(C)
+    spec = ((2, 3), (3, 1), torch.float32)
+    args = (1, 1, ctypes.addressof(d), d, 0)  # addresses that nothing calls
+    plan = calls.Plan(*args, (x, None), (spec, spec), (0, -1, -2))
+    assert calls.run([], 1, 0, 0, x, None) is None
+    assert calls.run([plan], 1, 0, 0, x, None) is None  # a CPU tensor
+    assert calls.run([plan], 1, 1, 0, x, None) is None  # another device's handle
+    assert calls.run([plan], 0, 0, 0, x, None) is None  # no handle
+    assert calls.run([plan, object()], 1, 0, 0, x) is None
+    assert calls.run([plan], 1, 0, 0, x, 5) is None
+    for ins, outs, slots in (((x,) * 6, (spec,), (0, -1, -1)), ((x,), (spec,), (0, -1)), ((x,), (spec,), (1, -1, -1)),
+                             ((x,), (spec,), (0, -1, -2)), ((3,), (spec,), (0, -1, -1)), ((x,), (((2,), (1, 1), torch.float32),), (0, -1, -1)),
+                             ((x,), (((2,), (1,), 5),), (0, -1, -1))):
+        with pytest.raises(ValueError):
+            calls.Plan(*args, ins, outs, slots)
+    with pytest.raises(TypeError):
+        calls.run()
+    with pytest.raises(TypeError):
+        calls.run((plan,), 1, 0, 0, x, None)
+    with pytest.raises(TypeError):
+        calls.Plan(*args, [x], (spec,), (0, -1, -1))

@@ -690,3 +690,88 @@ def test_long_offsets(ob, ctx):
     y = ob.MatMulBlockScaled(dtype=torch.bfloat16).compute([q, s, b, sb], ctx)[0]
     check_mm(y[-3:], q[-3:], s[-3:], b, sb, None, False, torch.bfloat16)
     assert (y[:-3] == 0).all()
+
+
+@pytest.fixture(params=[True, False], ids=["native_calls", "ctypes"])
+def calls(ob, request, monkeypatch):
+    """With the module for repeated calls, and without it."""
+    if request.param:
+        assert ob.ops._calls is not None, "onnx-rs_b200/_calls.so is not built"
+    else:
+        monkeypatch.setattr(ob.ops, "_calls", None)
+    return request.param
+
+
+def test_repeated_calls(ob, ctx, calls):
+    """Layouts in turn through one operator: each call's outputs are its own, and the first's bits."""
+    norm, quant = ob.RMSNormalization(1e-6, quantize=True), ob.QuantizeBlocks()
+    weights, mm = ob.QuantizeBlocks(128), ob.MatMulBlockScaled(torch.bfloat16, relu=True)
+    b, sb = weights.compute([normal((300, 640), 9)], ctx)
+    bias = normal((300,), 10)
+    seen = {}
+    for turn in range(3):
+        for i, (lead, res) in enumerate((((1,), True), ((40,), False), ((2, 3), True), ((300,), True))):
+            x, r = normal((*lead, 640), i, torch.bfloat16), normal((*lead, 640), 50 + i, torch.bfloat16)
+            w = normal((640,), 99, torch.bfloat16)
+            out = norm.compute([x, w], ctx, residual=r if res else None)
+            check_norm(out, x, r if res else None, w, 1e-6, True)
+            out += quant.compute([x[..., :500]], ctx)
+            out += mm.compute([out[0], out[1], b, sb] + ([bias] if i % 2 else []), ctx)
+            flat = [t.reshape(-1, t.shape[-1]) for t in (out[-1], out[0], out[1])]
+            check_mm(*flat, b, sb, bias if i % 2 else None, True, torch.bfloat16)
+            layout = [(t.shape, t.stride(), t.dtype) for t in out]
+            first = seen.setdefault(i, (out, layout))
+            assert layout == first[1]
+            if turn:
+                for t, f in zip(out, first[0]):
+                    assert t.data_ptr() != f.data_ptr()
+                    assert torch.equal(t.contiguous().view(torch.uint8), f.contiguous().view(torch.uint8))
+    assert bool(norm.__dict__.get("_plans")) == calls
+
+
+def test_repeated_calls_are_checked(ob, ctx, calls):
+    """What differs from the layouts seen before is checked as a first call is."""
+    x, w = normal((4, 256), 1), normal((256,), 2)
+    norm, mm = ob.RMSNormalization(), ob.MatMulBlockScaled()
+    a, sa, b, sb = operands(4, 8, 256, 1)
+    for _ in range(2):
+        norm.compute([x, w], ctx)
+        mm.compute([a, sa, b, sb], ctx)
+    for bad in ([x, w[:128]], [x.cpu(), w], [x, w.cpu()], [x.to(torch.int32), w], [x.t().contiguous().t(), w], [x[0, 0], w]):
+        with pytest.raises(ob.ValidationError):
+            norm.compute(bad, ctx)
+    with pytest.raises(ob.ValidationError):
+        norm.compute([x, w], ctx, residual=x[:2])
+    for bad in ([a, sa[:, :1], b, sb], [a, sa, b[:, :128], sb], [a, sa, b, sb, normal((7,), 1)], [a.float(), sa, b, sb]):
+        with pytest.raises(ob.ValidationError):
+            mm.compute(bad, ctx)
+    out = norm.compute([torch.nn.Parameter(x), torch.nn.Parameter(w)], ctx)[0]
+    assert not out.requires_grad
+    check_norm([out], x, None, w, 1e-5, False)
+    with torch.inference_mode():
+        check_norm(norm.compute([x, w], ctx), x, None, w, 1e-5, False)
+    h = ob.Handle(0)
+    other = ob.ExecutionContext(h)
+    check_norm(norm.compute([x, w], other), x, None, w, 1e-5, False)
+    h.close()
+    with pytest.raises(ob.OnnxB200Error):
+        norm.compute([x, w], other)
+    check_norm(norm.compute([x, w], ctx), x, None, w, 1e-5, False)
+
+
+def test_repeated_calls_on_streams(ob, calls):
+    """A handle on its own stream, on torch's, and torch on others: always in order with torch's current stream."""
+    w = torch.ones(2048, device="cuda")
+    for torch_stream in (True, False):
+        with ob.Handle(0, torch_stream=torch_stream) as h:
+            ctx, norm = ob.ExecutionContext(h), ob.RMSNormalization()
+            for stream in (None, torch.cuda.Stream(), None, torch.cuda.Stream()):
+                with torch.cuda.stream(stream):
+                    x = normal((512, 2048), 3)
+                    eye = torch.eye(2048, device="cuda")
+                    for _ in range(8):  # a producer that is still running when the call is made
+                        x = x @ eye
+                    y = norm.compute([x, w], ctx)[0].clone()
+                    torch.cuda.current_stream().synchronize()
+                    check_norm([y], x, None, w, 1e-5, False)
+            torch.cuda.synchronize()
