@@ -234,9 +234,106 @@ __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, CH == 4 && 
     if (at(c) < n8) store_e4m3(q + at(c) * 8, h[c], inv[c]);
 }
 
+// Any alignment, up to 4096 columns: one row per thread block, blocks of 128 columns
+// dealt to its warps (NB each, four columns a lane), all elements of x, the residual
+// and the weight on their way before the first is used; h stays in registers.  Bound
+// by its element accesses: 4096 x 1001 fp16 with residual and e4m3 output (29 MB)
+// 13.7 us, fp32 without (33 MB) 9.4 us.
+constexpr int kRowThreads = 512;
+template <typename T, typename W, int NB>
+__global__ void __launch_bounds__(kRowThreads, NB == 1 ? 4 : 2) rmsnorm_elem_kernel(const RmsNormArgs p) {
+  __shared__ float part[kRowThreads / 32];
+  pdl_begin();
+  const int64_t r = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const T* x = static_cast<const T*>(p.x) + r * p.ldx;
+  const W* w = static_cast<const W*>(p.weight);
+  auto block = [&](int c) { return c * warps + warp; };
+  auto at = [&](int c, int j) { return block(c) * kQBlock + j * 32 + lane; };
+  float h[NB][4];
+  {
+    T a[NB][4];
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[c][j] = at(c, j) < p.cols ? x[at(c, j)] : from_f32<T>(0.f);
+    if (p.res) {
+      const T* res = static_cast<const T*>(p.res) + r * p.ldr;
+      T b[NB][4];
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[c][j] = at(c, j) < p.cols ? res[at(c, j)] : from_f32<T>(0.f);
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[c][j] = to_f32(a[c][j]) + to_f32(b[c][j]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[c][j] = to_f32(a[c][j]);
+    }
+  }
+  W g[NB][4];
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[c][j] = at(c, j) < p.cols ? w[at(c, j)] : from_f32<W>(0.f);
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ss = fmaf(h[c][j], h[c][j], ss);
+  ss = warp_sum(ss);
+  if (lane == 0) part[warp] = ss;
+  if (p.sum) {
+    T* sum = static_cast<T*>(p.sum) + r * p.lds;
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at(c, j) < p.cols) sum[at(c, j)] = from_f32<T>(h[c][j]);
+  }
+  __syncthreads();
+  float tot = 0.f;
+  for (int i = 0; i < warps; ++i) tot += part[i];
+  const float rstd = 1.f / sqrtf(tot / (float)p.cols + p.eps);
+  float amax[NB];
+#pragma unroll
+  for (int c = 0; c < NB; ++c) {
+    amax[c] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[c][j] = h[c][j] * rstd * to_f32(g[c][j]);
+      if (at(c, j) < p.cols) amax[c] = max_nan(amax[c], fabsf(h[c][j]));
+    }
+  }
+  if (p.out_type != kE4M3) {
+    T* y = static_cast<T*>(p.y) + r * p.ldy;
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (at(c, j) < p.cols) y[at(c, j)] = from_f32<T>(h[c][j]);
+    return;
+  }
+  uint8_t* q = static_cast<uint8_t*>(p.y) + r * p.ldy;
+#pragma unroll
+  for (int c = 0; c < NB; ++c) amax[c] = warp_max_nan(amax[c]);
+#pragma unroll
+  for (int c = 0; c < NB; ++c) {
+    float scale, inv;
+    block_scale(amax[c], scale, inv);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (at(c, j) < p.cols) q[at(c, j)] = to_e4m3(h[c][j] * inv);
+    if (lane == 0 && block(c) * kQBlock < p.cols) p.y_scale[r * p.ys_row + block(c) * p.ys_block] = scale;
+  }
+}
+
 // Any alignment and width: one row per block, the row's fp32 sum x + residual held
 // in shared memory.
-constexpr int kRowThreads = 512;
 template <typename T, typename W>
 __global__ void __launch_bounds__(kRowThreads) rmsnorm_row_kernel(const RmsNormArgs p) {
   extern __shared__ float row[];
@@ -476,6 +573,12 @@ int rmsnorm_launch(const RmsNormArgs& a, int num_sms, cudaStream_t st) {
       const bool vec = a.cols % 8 == 0 && a.cols <= 4 * 512 * 8 && on_grid(a.x, a.ldx, sizeof(T), 16) &&
                        (!a.res || on_grid(a.res, a.ldr, sizeof(T), 16)) && (!a.sum || on_grid(a.sum, a.lds, sizeof(T), 16)) &&
                        on_grid(a.weight, 0, sizeof(W), 16) && on_grid(a.y, a.ldy, quant ? 1 : sizeof(T), quant ? 8 : 16);
+      // Short rows off the grid stay in registers, a warp for one or two blocks of columns
+      // (4096 x 1001 fp16: 13.7 us, 22.6 in shared memory; 4096 x 3001 bf16 28.4 and 30.0);
+      // with four a warp the registers left too few warps (8192 x 8001: 167 us and 138).
+      const int nb = (a.cols + kQBlock - 1) / kQBlock;
+      if (!vec && nb <= 16) return launch_pdl(rmsnorm_elem_kernel<T, W, 1>, (unsigned)a.rows, nb * 32, 0, st, a);
+      if (!vec && nb <= 32) return launch_pdl(rmsnorm_elem_kernel<T, W, 2>, (unsigned)a.rows, (nb + 1) / 2 * 32, 0, st, a);
       if (!vec) {
         const int smem = a.cols * (int)sizeof(float);
         if (smem > 48 * 1024 - 64) {

@@ -775,3 +775,35 @@ def test_repeated_calls_on_streams(ob, calls):
                     torch.cuda.current_stream().synchronize()
                     check_norm([y], x, None, w, 1e-5, False)
             torch.cuda.synchronize()
+
+
+# The error bound of norm_slack holds here too: a thread adds 4 or 8 squares, a shuffle 5 and the row at most 16
+# parts, 29 roundings at most of a sum whose square root halves them: 15 U at 4096 columns, where norm_slack has 22,
+# 13 at 2048 (18) and 6 at 130 (14.5), with 5 for the division, root and products.
+@pytest.mark.parametrize("residual,quantize", [(False, False), (True, True)])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols", [(700, 2), (3, 127), (2, 129), (310, 1025), (2, 2047), (3, 2049), (305, 3001), (2, 3968),
+                                       (2, 4095), (3, 4097)])
+def test_rmsnorm_off_the_grid(ob, ctx, rows, cols, t, residual, quantize):
+    """Rows of every length around what a warp and a thread block hold, none on a 16-byte boundary for long."""
+    x = normal((rows, cols + 1), rows + cols, t)[:, 1:]
+    r = 3 * normal((rows, cols), 7, t) if residual else None
+    w = (1 + 0.3 * normal((cols + 1,), 9)).to(t)[1:]
+    out = ob.RMSNormalization(epsilon=1e-5, quantize=quantize).compute([x, w], ctx, residual=r)
+    check_norm(out, x, r, w, 1e-5, quantize)
+
+
+def test_rmsnorm_off_the_grid_non_finite(ob, ctx):
+    """As on the grid: a NaN or an infinity stays in its row, a zero row is zero."""
+    for cols in (381, 2501):
+        x = normal((5, cols), 1)
+        x[1] = 0
+        x[2, 5] = float("inf")
+        x[3, cols - 1] = float("nan")
+        w = torch.ones(cols, device="cuda")
+        y = ob.RMSNormalization().compute([x, w], ctx)[0]
+        assert (y[1] == 0).all() and torch.isnan(y[2, 5]) and (y[2, 6:] == 0).all() and torch.isnan(y[3]).all()
+        check_norm([y[[0, 4]]], x[[0, 4]], None, w, 1e-5, False)
+        q, s = ob.RMSNormalization(quantize=True).compute([x, w], ctx)
+        assert (q[1].float() == 0).all() and torch.isfinite(s[1]).all()
+        assert not torch.isfinite(s[2, 0]) and torch.isfinite(s[2, 1:]).all() and not torch.isfinite(s[3]).any()
