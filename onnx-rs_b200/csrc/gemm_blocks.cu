@@ -8,6 +8,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "blocks.cuh"
 #include "ptx.cuh"
@@ -945,6 +946,48 @@ bool encode_out(const MatmulBlocksArgs& a, CUtensorMap* map) {
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <int BN>
+cudaLaunchConfig_t pair_config(unsigned grid, int split, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = PairLayout<BN>::kBytes;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2u * split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
+// Tiles that run at once where `split` pairs share each: clusters of 2 * split CTAs do not
+// cross the groups of SMs that the GPU is made of, so that fewer fit than its SMs would
+// hold.  A device's answer never changes: asked once.
+template <typename T>
+int split_tiles(int split) {
+  static std::atomic<int> known[16][2];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 16) return 0;
+  std::atomic<int>& k = known[dev][split == 4];
+  int v = k.load(std::memory_order_relaxed);
+  if (v == 0) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = pair_config<128>(2u * split, split, attr);
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (opt_in<matmul_blocks_pair_kernel<T, 128, true>>(PairLayout<128>::kBytes) != 0 ||
+        cudaOccupancyMaxActiveClusters(&n, matmul_blocks_pair_kernel<T, 128, true>, &cfg) != cudaSuccess) {
+      cudaGetLastError();  // no reason for the launch without sharing to fail
+      return 0;
+    }
+    v = n + 1;  // 0: not asked yet
+    k.store(v, std::memory_order_relaxed);
+  }
+  return v - 1;
+}
+
 // split: pairs that share a tile (1, 2 or 4; BN == 128).
 template <typename T, int BN, bool SPLIT = false>
 int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st, int split = 1) {
@@ -956,19 +999,9 @@ int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st, int spl
   int rc = opt_in<matmul_blocks_pair_kernel<T, BN, SPLIT>>(L::kBytes);
   if (rc) return rc;
   const int tiles = ((a.m + 255) / 256) * ((a.n + BN - 1) / BN);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2u * split * (SPLIT ? tiles : std::min(tiles, num_sms / 2)));
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = L::kBytes;
-  cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2u * split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cudaLaunchConfig_t cfg = pair_config<BN>(2u * split * (SPLIT ? tiles : std::min(tiles, num_sms / 2)), split, attr);
+  cfg.stream = st;
   return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN, SPLIT>, a, ma, mb, my, tma_out, split);
 }
 
@@ -992,12 +1025,15 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       // 8192: 15.3 and 20.4 us, 512 x 8192: 23.4 and 21.4 us, 4096 x 4096: 70.6 and 67.2 us).
       const int64_t tm = (a.m + 255) / 256, pairs = num_sms / 2;
       const int64_t wide = (tm * ((a.n + 255) / 256) + pairs - 1) / pairs, narrow = (tm * ((a.n + 127) / 128) + pairs - 1) / pairs;
-      // Few tiles: two or four pairs share one, each a slice of k of four blocks at
-      // least (128 x 4096 x 14336: 23.2 us with two, 36 with one; 256 x 4096 x 4096: 13.3
-      // and 14.5).
+      // Few tiles: two or four pairs share one, where all run at once (with one, two and
+      // four: 256 x 1024 x 4096 13.2, 12.3 and 10.6 us; 100 x 1000 x 14336 30.9, 21.6 and
+      // 15.5; but 200 x 2048 x 4096, whose 16 clusters of eight CTAs take two turns, 13.3,
+      // 12.5 and 19.2, and 256 x 4608 x 4096 13.8, 23.1 and 28.6) and k is long enough to
+      // pay for the join (256 x 1280 x 2048: 9.0, 9.7 and 9.0; 256 x 2560 x 2560 10.8 and
+      // 11.3 with one and two).
       const int64_t tiles = tm * ((a.n + 127) / 128);
-      if (tiles * 4 <= pairs && kbs >= 16) return launch_pair<T, 128, true>(a, num_sms, st, 4);
-      if (tiles * 2 <= pairs && kbs >= 8) return launch_pair<T, 128, true>(a, num_sms, st, 2);
+      if (tiles * 4 <= pairs && kbs >= 16 && tiles <= split_tiles<T>(4)) return launch_pair<T, 128, true>(a, num_sms, st, 4);
+      if (tiles * 2 <= pairs && kbs >= 28 && tiles <= split_tiles<T>(2)) return launch_pair<T, 128, true>(a, num_sms, st, 2);
       return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
     }
     const size_t vec_smem = (size_t)a.m * ((a.k + 15) / 16 * 32 + kbs * 4);

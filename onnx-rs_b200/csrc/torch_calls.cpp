@@ -3,8 +3,8 @@
 // An operator's first call with tensors of some layout checks them, fills a
 // descriptor and knows its outputs' layouts (ops.py).  A Plan keeps that, and
 // run() makes the next call with the same layouts from it: compares the layouts,
-// allocates the outputs and calls the C entry.  The host's share of a call: 6.3 us
-// (norm with residual and e4m3 output, three outputs), 5.2 (quantise), 4.6 (product);
+// allocates the outputs and calls the C entry.  The host's share of a call: 5.9 us
+// (norm with residual and e4m3 output, three outputs), 4.9 (quantise), 4.4 (product);
 // through ctypes and torch's Python functions 10.8, 7.3 and 8.6.  The launch itself is
 // 2.3 of them, each output 0.5.
 //

@@ -640,6 +640,7 @@ class _Described:
     whose layouts were seen before is made there (csrc/torch_calls.cpp)."""
     entry = None   # name of the C entry
     slots = ()     # its pointers behind the descriptor: an input, or -1 - an output
+    _plans = None
 
     def __setattr__(self, name, value):
         """A changed setting: what was kept does not hold any more."""
@@ -652,10 +653,9 @@ class _Described:
         return {k: v for k, v in self.__dict__.items() if k not in ("_kept", "_plans")}
 
     def _call(self, h, *tensors):
-        plans = self.__dict__.get("_plans")
-        if plans and h.ptr:
-            out = _calls.run(plans, h.ptr.value, h.device, h.own_stream_ptr, *tensors)
-            if out.__class__ is list:
+        if self._plans:
+            out = _calls.run(self._plans, h.address, h.device, h.own_stream_ptr, *tensors)
+            if type(out) is list:
                 return out
             if out is not None:
                 h.check(out, self.op_type)
@@ -687,9 +687,11 @@ class _Described:
         present = [i for i, spec in enumerate(specs) if spec is not None]
         slots = tuple((s if tensors[s] is not None else None) if s >= 0 else
                       (-1 - present.index(-1 - s) if specs[-1 - s] is not None else None) for s in self.slots)
+        if self._plans is None:
+            self.__dict__["_plans"] = []
         plan = _calls.Plan(_address(getattr(C.lib(), self.entry)), _address(C.lib().onnxb200_get_stream),
                            ctypes.addressof(desc), desc, h.device, tensors, tuple(specs[i] for i in present), slots)
-        self.__dict__.setdefault("_plans", []).insert(0, plan)
+        self._plans.insert(0, plan)
         return got
 
 
@@ -871,7 +873,9 @@ class MatMulBlockScaled(_Described, Operator):
         return d, (_dense((*a.shape[:-1], n), self.dtype),), relaid
 
     def compute(self, inputs, ctx):
-        return self._call(ctx.handle, *inputs[:4], inputs[4] if len(inputs) > 4 else None)
+        a, a_scale, b, b_scale = inputs[:4]
+        bias = inputs[4] if len(inputs) > 4 else None
+        return self._call(ctx.handle, a, a_scale, b, b_scale, bias)
 
 
 # --------------------------------------------------------------------------- registry

@@ -97,6 +97,7 @@ class Handle:
             raise_for(rc, f"onnxb200_create(device={device}) failed: "
                           f"{self.lib.onnxb200_status_string(rc).decode()}")
         self.ptr = ptr
+        self.address = ptr.value
         self.own_stream_ptr = self.stream_ptr
         if torch_stream:
             s = torch.cuda.current_stream(device)
@@ -126,6 +127,7 @@ class Handle:
         if getattr(self, "ptr", None):
             self.lib.onnxb200_destroy(self.ptr)
             self.ptr = None
+            self.address = 0
 
     def __del__(self):
         try:

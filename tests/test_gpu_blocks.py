@@ -807,3 +807,40 @@ def test_rmsnorm_off_the_grid_non_finite(ob, ctx):
         q, s = ob.RMSNormalization(quantize=True).compute([x, w], ctx)
         assert (q[1].float() == 0).all() and torch.isfinite(s[1]).all()
         assert not torch.isfinite(s[2, 0]) and torch.isfinite(s[2, 1:]).all() and not torch.isfinite(s[3]).any()
+
+
+@pytest.mark.parametrize("m,n,k", [(256, 512, 2560), (100, 1000, 2048), (70, 1700, 4000), (200, 2048, 4096), (129, 2560, 3700),
+                                   (512, 2304, 4096), (256, 4200, 3600), (256, 4608, 3600)])
+def test_product_with_few_tiles(ob, ctx, m, n, k):
+    """Tiles shared by one, two or four pairs of thread blocks, up to and past what runs at once."""
+    a, sa, b, sb = operands(m, n, k, m + n)
+    bias = normal((n,), 3)
+    y = ob.MatMulBlockScaled(torch.float32, relu=True).compute([a, sa, b, sb, bias], ctx)[0]
+    check_mm(y, a, sa, b, sb, bias, True, torch.float32)
+    assert torch.equal(y, ob.MatMulBlockScaled(torch.float32, relu=True).compute([a, sa, b, sb, bias], ctx)[0])
+
+
+def test_shared_tiles_first_inside_a_capture():
+    """What is asked of the device once, before tiles are shared, may be asked during a capture."""
+    import subprocess
+    import sys
+    code = """
+import importlib, torch
+ob = importlib.import_module("onnx-rs_b200")
+ctx = ob.ExecutionContext(ob.Handle(0))
+x, wt = torch.randn(100, 4096, device="cuda"), torch.randn(2000, 4096, device="cuda")
+torch.cuda.synchronize()
+def run():
+    (q, s), (b, sb) = ob.QuantizeBlocks().compute([x], ctx), ob.QuantizeBlocks(128).compute([wt], ctx)
+    return ob.MatMulBlockScaled().compute([q, s, b[:400], sb[:4], ], ctx) + ob.MatMulBlockScaled().compute([q, s, b, sb], ctx)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+torch.cuda.synchronize()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) and torch.isfinite(x).all() for x, y in zip(got, want))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
