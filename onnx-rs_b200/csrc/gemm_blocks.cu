@@ -900,6 +900,50 @@ bool encode_rows(const uint8_t* q, int rows, int k, int64_t ld, int box, CUtenso
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+cudaLaunchConfig_t cluster_config(unsigned grid, unsigned cluster, int threads, int smem, cudaLaunchAttribute (&attr)[2]) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
+// Clusters of 4 or 8 CTAs that run at once: a cluster does not cross the groups of SMs that
+// the GPU is made of, so that fewer fit than its SMs would hold.  A device's answer never
+// changes: asked once, of a kernel that does nothing in CTAs of the same size (of one that
+// takes tensor memory it is given for one CTA per SM, though two run).
+template <int THREADS, int PER_SM, int TAG>
+__global__ void __launch_bounds__(THREADS, PER_SM) same_size_kernel() {}
+template <auto KERNEL>
+int clusters_at_once(unsigned cluster, int threads, int smem) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> known[kMaxDevices][2];  // plus one; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  std::atomic<int>& k = known[dev][cluster == 8];
+  int v = k.load(std::memory_order_relaxed);
+  if (v == 0) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = cluster_config(cluster, cluster, threads, smem, attr);
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (opt_in<KERNEL>(smem) != 0 || cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
+      cudaGetLastError();  // no reason for the launch of smaller clusters to fail
+      return 0;
+    }
+    v = n + 1;
+    k.store(v, std::memory_order_relaxed);
+  }
+  return v - 1;
+}
+
 template <typename T, int M>
 int launch_vec(const MatmulBlocksArgs& a, size_t smem, cudaStream_t st) {
   if (smem > 48 * 1024) {
@@ -918,20 +962,26 @@ int launch_rows(const MatmulBlocksArgs& a, int split, cudaStream_t st) {
     return (int)cudaErrorInvalidValue;
   int rc = opt_in<matmul_blocks_rows_kernel<T, BN>>(L::kBytes);
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.n + 127) / 128) * split);
-  cfg.blockDim = dim3(kRowsThreads);
-  cfg.dynamicSmemBytes = L::kBytes;
-  cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cudaLaunchConfig_t cfg = cluster_config((unsigned)((a.n + 127) / 128) * split, (unsigned)split, kRowsThreads, L::kBytes, attr);
+  cfg.stream = st;
   return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_rows_kernel<T, BN>, a, w, x, split);
+}
+
+// Split k over CTAs until they fill the GPU's SMs once or twice, two blocks each at
+// least; the first split also pays for the clusters (16 x 4096 x 4096 with 32
+// tiles: 12.9, 10.8, 8.9 and 8.7 us with 1, 2, 4 and 8 CTAs a tile; 16 x 14336 x
+// 4096 with 112: 15.1, 16.4, 19.9; 17 x 1000 x 2048 with 8: 9.1, 9.2, 7.2, 5.9), and
+// no further than the clusters run at once (16 x 9472 x 4096, whose 74 clusters of
+// four take two turns: 13.0, 13.2, 16.6).
+template <typename T, int BN>
+int rows_split(const MatmulBlocksArgs& a, int num_sms) {
+  const int tiles = (a.n + 127) / 128, kbs = (a.k + kQBlock - 1) / kQBlock;
+  int split = tiles * 4 <= num_sms * 3 && kbs >= 4 ? 2 : 1;
+  while (split > 1 && split < 8 && tiles * split <= num_sms && kbs >= split * 4 &&
+         tiles <= clusters_at_once<same_size_kernel<kRowsThreads, 2, BN>>(2u * split, kRowsThreads, RowsLayout<BN>::kBytes))
+    split *= 2;
+  return split;
 }
 
 // Boxes of 32 rows by 128 bytes of y, for the stores; false where TMA cannot write.
@@ -946,48 +996,6 @@ bool encode_out(const MatmulBlocksArgs& a, CUtensorMap* map) {
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN>
-cudaLaunchConfig_t pair_config(unsigned grid, int split, cudaLaunchAttribute (&attr)[2]) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = PairLayout<BN>::kBytes;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2u * split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cfg;
-}
-
-// Tiles that run at once where `split` pairs share each: clusters of 2 * split CTAs do not
-// cross the groups of SMs that the GPU is made of, so that fewer fit than its SMs would
-// hold.  A device's answer never changes: asked once.
-template <typename T>
-int split_tiles(int split) {
-  static std::atomic<int> known[16][2];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 16) return 0;
-  std::atomic<int>& k = known[dev][split == 4];
-  int v = k.load(std::memory_order_relaxed);
-  if (v == 0) {
-    cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t cfg = pair_config<128>(2u * split, split, attr);
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (opt_in<matmul_blocks_pair_kernel<T, 128, true>>(PairLayout<128>::kBytes) != 0 ||
-        cudaOccupancyMaxActiveClusters(&n, matmul_blocks_pair_kernel<T, 128, true>, &cfg) != cudaSuccess) {
-      cudaGetLastError();  // no reason for the launch without sharing to fail
-      return 0;
-    }
-    v = n + 1;  // 0: not asked yet
-    k.store(v, std::memory_order_relaxed);
-  }
-  return v - 1;
-}
-
 // split: pairs that share a tile (1, 2 or 4; BN == 128).
 template <typename T, int BN, bool SPLIT = false>
 int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st, int split = 1) {
@@ -1000,7 +1008,8 @@ int launch_pair(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st, int spl
   if (rc) return rc;
   const int tiles = ((a.m + 255) / 256) * ((a.n + BN - 1) / BN);
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = pair_config<BN>(2u * split * (SPLIT ? tiles : std::min(tiles, num_sms / 2)), split, attr);
+  cudaLaunchConfig_t cfg =
+      cluster_config(2u * split * (SPLIT ? tiles : std::min(tiles, num_sms / 2)), 2u * split, kPairThreads, L::kBytes, attr);
   cfg.stream = st;
   return (int)cudaLaunchKernelEx(&cfg, matmul_blocks_pair_kernel<T, BN, SPLIT>, a, ma, mb, my, tma_out, split);
 }
@@ -1032,23 +1041,19 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       // pay for the join (256 x 1280 x 2048: 9.0, 9.7 and 9.0; 256 x 2560 x 2560 10.8 and
       // 11.3 with one and two).
       const int64_t tiles = tm * ((a.n + 127) / 128);
-      if (tiles * 4 <= pairs && kbs >= 16 && tiles <= split_tiles<T>(4)) return launch_pair<T, 128, true>(a, num_sms, st, 4);
-      if (tiles * 2 <= pairs && kbs >= 28 && tiles <= split_tiles<T>(2)) return launch_pair<T, 128, true>(a, num_sms, st, 2);
+      auto at_once = [&](int s) {
+        return clusters_at_once<same_size_kernel<kPairThreads, 1, 128>>(2u * s, kPairThreads, PairLayout<128>::kBytes);
+      };
+      if (tiles * 4 <= pairs && kbs >= 16 && tiles <= at_once(4)) return launch_pair<T, 128, true>(a, num_sms, st, 4);
+      if (tiles * 2 <= pairs && kbs >= 28 && tiles <= at_once(2)) return launch_pair<T, 128, true>(a, num_sms, st, 2);
       return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
     }
     const size_t vec_smem = (size_t)a.m * ((a.k + 15) / 16 * 32 + kbs * 4);
     if (a.m <= 2 && vec_smem <= kVecMaxSmem)
       return a.m == 1 ? launch_vec<T, 1>(a, vec_smem, st) : launch_vec<T, 2>(a, vec_smem, st);
-    // Split k over CTAs until they fill the GPU's SMs once or twice, two blocks each at
-    // least; the first split also pays for the clusters (16 x 4096 x 4096 with 32
-    // tiles: 12.9, 10.8, 8.9 and 8.7 us with 1, 2, 4 and 8 CTAs a tile; 16 x 14336 x
-    // 4096 with 112: 15.1, 16.4, 19.9; 17 x 1000 x 2048 with 8: 9.1, 9.2, 7.2, 5.9).
-    const int tiles = (a.n + 127) / 128;
-    int split = tiles * 4 <= num_sms * 3 && kbs >= 4 ? 2 : 1;
-    while (split > 1 && split < 8 && tiles * split <= num_sms && kbs >= split * 4) split *= 2;
-    return a.m <= 16   ? launch_rows<T, 16>(a, split, st)
-           : a.m <= 32 ? launch_rows<T, 32>(a, split, st)
-                       : launch_rows<T, 64>(a, split, st);
+    return a.m <= 16   ? launch_rows<T, 16>(a, rows_split<T, 16>(a, num_sms), st)
+           : a.m <= 32 ? launch_rows<T, 32>(a, rows_split<T, 32>(a, num_sms), st)
+                       : launch_rows<T, 64>(a, rows_split<T, 64>(a, num_sms), st);
   });
 }
 
