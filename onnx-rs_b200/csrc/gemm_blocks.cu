@@ -434,15 +434,16 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 // walk the tiles, and a tile's stores (TMA, from shared memory) run under the
 // next tile's loads and MMAs.
 //
-// What bounds it: at 256 x 256 a block of 128 k's takes 710 cycles, of which the
-// MMAs need 512 (a pure stream of them measured 512, at 1.4 GHz under the power cap
-// 3.3 PFLOP/s).  With a quarter of the columns read and added it took 620, with half
-// of the operands loaded as well 600: the rest is the round trip MMA -> commit ->
-// reads -> arrival on the leader, which two accumulators per half do not cover, and
-// the clock, 1.2 to 1.4 GHz at the power cap.  TMEM is full, and so are the registers:
-// with sixteen columns in flight instead of 64 8192^3 took 523 instead of 503 us,
-// with the next block's first columns loaded under the last additions 600 (register
-// moves), with sixteen warps and half the totals each 580 (spills).
+// What bounds it: at 256 x 256 a block of 128 k's takes 690 cycles, of which the MMAs
+// need 512 (a pure stream of them measured 512, at 1.4 GHz under the power cap 3.3
+// PFLOP/s).  With a quarter of the MMAs it still takes 685, with a quarter of the
+// columns read and added 520: the epilogue warps set it, by latencies (a wait that is
+// answered at once 95 cycles, the reads of two times 64 columns 190, the last additions
+// 105) that two warps per scheduler do not cover, and the clock, 1.2 to 1.4 GHz at the
+// power cap.  TMEM is full, and so are the registers: with sixteen columns in flight
+// instead of 64 8192^3 took 523 instead of 503 us, with the next block's first columns
+// loaded under the last additions 527 to 600 (register moves), with sixteen warps and
+// half the totals each 580 (spills); a second warp to issue the MMAs changed nothing.
 // Run without a pause (1.24 to 1.5 GHz): 8192^3 bf16 508 us, 2.16 PFLOP/s; 4096^3 72
 // us; 8192 x 8192 x 1024 80 us (its tiles' output is a sixth); after idle, at higher
 // clocks, 8192^3 435 us.  200 x 8192 x 4096 (256 x 128 tiles, 36 MB) 15 us, its loop
