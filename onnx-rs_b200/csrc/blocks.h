@@ -52,6 +52,13 @@ struct MatmulBlocksArgs {
   int out_type, relu;
   int* status;         // device status word (ONNXB200_ERR_* on failure)
 };
+// The CUDA-core product for one or two rows of a keeps them whole in shared memory, as
+// fp16 and with a scale per block of k.  Bytes in 64 bits: k goes up to 2^31.
+constexpr int64_t kVecMaxSmem = 100 * 1024;  // two thread blocks per SM; longer rows go to the tensor cores
+constexpr int64_t matmul_vec_smem(int m, int k) {
+  return m * (((int64_t)k + 15) / 16 * 32 + ((int64_t)k + kQBlock - 1) / kQBlock * 4);
+}
+constexpr bool matmul_takes_vec(int m, int k) { return m <= 2 && matmul_vec_smem(m, k) <= kVecMaxSmem; }
 int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t stream);
 
 }  // namespace ob2

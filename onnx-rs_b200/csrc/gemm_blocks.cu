@@ -102,7 +102,6 @@ __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlo
 // MB; 8.1 in the kernel for few rows), 1 x 8192 x 8192 15.4 us (4.4 TB/s), 2 x 4096 x
 // 4096 8.3 us, and four rows 10.9, more than below.
 constexpr int kVecWarps = 8, kVecRows = 2, kVecUnroll = 4;
-constexpr int kVecMaxSmem = 100 * 1024;  // two blocks per SM; longer rows of a go to the tensor cores
 template <typename T, int M>
 __global__ void __launch_bounds__(kVecWarps * 32) matmul_blocks_vec_kernel(const MatmulBlocksArgs p) {
   extern __shared__ uint4 va[];  // [M][2][chunks] eight fp16 of a; then [M][blocks] scales
@@ -946,9 +945,10 @@ int clusters_at_once(unsigned cluster, int threads, int smem) {
 }
 
 template <typename T, int M>
-int launch_vec(const MatmulBlocksArgs& a, size_t smem, cudaStream_t st) {
+int launch_vec(const MatmulBlocksArgs& a, cudaStream_t st) {
+  const size_t smem = (size_t)matmul_vec_smem(M, a.k);
   if (smem > 48 * 1024) {
-    const int rc = opt_in<matmul_blocks_vec_kernel<T, M>>(kVecMaxSmem);
+    const int rc = opt_in<matmul_blocks_vec_kernel<T, M>>((int)kVecMaxSmem);
     if (rc) return rc;
   }
   const unsigned per = kVecWarps * kVecRows;
@@ -1049,9 +1049,7 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       if (tiles * 2 <= pairs && kbs >= 28 && tiles <= at_once(2)) return launch_pair<T, 128, true>(a, num_sms, st, 2);
       return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
     }
-    const size_t vec_smem = (size_t)a.m * ((a.k + 15) / 16 * 32 + kbs * 4);
-    if (a.m <= 2 && vec_smem <= kVecMaxSmem)
-      return a.m == 1 ? launch_vec<T, 1>(a, vec_smem, st) : launch_vec<T, 2>(a, vec_smem, st);
+    if (matmul_takes_vec(a.m, a.k)) return a.m == 1 ? launch_vec<T, 1>(a, st) : launch_vec<T, 2>(a, st);
     return a.m <= 16   ? launch_rows<T, 16>(a, rows_split<T, 16>(a, num_sms), st)
            : a.m <= 32 ? launch_rows<T, 32>(a, rows_split<T, 32>(a, num_sms), st)
                        : launch_rows<T, 64>(a, rows_split<T, 64>(a, num_sms), st);
