@@ -67,7 +67,7 @@ bool resolve_scale(int64_t* row, int64_t* block, int64_t rows, int64_t blocks, b
   const bool one_row = rows <= 1, one_block = blocks <= 1;
   if ((!one_row && *row == 0) || (!one_block && *block == 0)) return false;
   if (one_row || one_block) return true;
-  return *row >= *block * blocks || *block >= *row * rows;
+  return *row / blocks >= *block || *block / rows >= *row;  // products of the two pass 64 bits
 }
 int64_t blocks_of(int64_t v) { return (v + kQBlock - 1) / kQBlock; }
 

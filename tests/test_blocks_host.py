@@ -245,3 +245,18 @@ def test_module_for_repeated_calls(ob, C):
         calls.run((plan,), 1, 0, 0, x, None)
     with pytest.raises(TypeError):
         calls.Plan(*args, [x], (spec,), (0, -1, -1))
+
+
+@pytest.mark.parametrize("rows,row,block", [(1 << 28, 1 << 36, 1 << 36), (1 << 30, 1 << 34, 1 << 34),
+                                            (1 << 27, 1 << 37, 1 << 37)])
+def test_scales_that_overlap_far_apart(C, rows, row, block):
+    """Scales (i, j) and (i + 1, j - 1) in one place, with strides whose products pass 64 bits."""
+    assert call_norm(C, norm_desc(C, rows=rows, out_type=E4M3, y_scale_row=row, y_scale_block=block)) == C.ERR_VALIDATION
+    assert call_quant(C, quant_desc(C, rows=rows, scale_row=row, scale_block=block)) == C.ERR_VALIDATION
+
+
+def test_scales_side_by_side_at_the_edge(C):
+    """The closest strides that do not overlap are taken, both ways round."""
+    for row, block in ((2, 1), (1, 4), (3, 1), (1, 5), (1 << 37, 1 << 36), (1 << 35, 1 << 37)):
+        assert call_norm(C, norm_desc(C, out_type=E4M3, y_scale_row=row, y_scale_block=block)) == C.ERR_INVALID_ARGUMENT
+        assert call_quant(C, quant_desc(C, scale_row=row, scale_block=block)) == C.ERR_INVALID_ARGUMENT
