@@ -18,7 +18,8 @@ from __future__ import annotations
 import ctypes
 import math
 import os
-from typing import Dict, List, Optional, Sequence
+import threading
+from typing import Dict, List, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -634,32 +635,47 @@ def _layout(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
+class _Kept(NamedTuple):
+    """What an operator keeps of a call: nothing of it depends on where the elements are."""
+    desc: ctypes.Structure
+    specs: tuple     # (shape, strides, dtype) of each output, None where there is none
+    relaid: Sequence  # (input, function that lays it out anew) on every call
+    plan: object     # of the native module, or None
+
+
+_keeping = threading.Lock()  # held to publish what operators keep, never during a call's own work
+
+
 class _Described:
     """Operators whose checks, descriptors and output layouts are kept from call to call, by the
     operator's settings and the layout of the inputs.  Where the native module _calls is built, a call
-    whose layouts were seen before is made there (csrc/torch_calls.cpp)."""
+    whose layouts were seen before is made there (csrc/torch_calls.cpp).  Threads may share an operator:
+    _plans is replaced as a whole, together with what _kept holds, and what a call made under settings
+    that have changed since is not kept."""
     entry = None   # name of the C entry
     slots = ()     # its pointers behind the descriptor: an input, or -1 - an output
     _plans = None
 
     def __setattr__(self, name, value):
         """A changed setting: what was kept does not hold any more."""
-        object.__setattr__(self, name, value)
-        self.__dict__.pop("_kept", None)
-        self.__dict__.pop("_plans", None)
+        with _keeping:
+            object.__setattr__(self, name, value)
+            self.__dict__.pop("_kept", None)
+            self.__dict__.pop("_plans", None)
 
     def __getstate__(self):
         # pointers are neither copied nor pickled
         return {k: v for k, v in self.__dict__.items() if k not in ("_kept", "_plans")}
 
     def _call(self, h, *tensors):
-        if self._plans:
-            out = _calls.run(self._plans, h.address, h.device, h.own_stream_ptr, *tensors)
+        plans = self._plans
+        if plans:
+            out = _calls.run(plans, h.address, h.device, h.own_stream_ptr, *tensors)
             if type(out) is list:
                 return out
             if out is not None:
                 h.check(out, self.op_type)
-        desc, specs, relaid = self._described(h, self._prepare, *tensors)
+        desc, specs, relaid, _ = self._described(h, self._prepare, *tensors)
         for i, lay in relaid:
             tensors = (*tensors[:i], lay(tensors[i]), *tensors[i + 1:])
         new = _new_on(tensors[0].device)
@@ -669,30 +685,31 @@ class _Described:
         return [t for t in outs if t is not None]
 
     def _described(self, handle, make, *tensors):
+        kept = self.__dict__.setdefault("_kept", {})  # before the settings are read: a change takes it away
         key = (handle.device, self._settings(), *map(_layout, tensors))
-        kept = self.__dict__.setdefault("_kept", {})
         got = kept.get(key)
         if got is None:
-            if len(kept) >= 64:
-                kept.clear()
-                self.__dict__.pop("_plans", None)
-            got = kept[key] = make(handle, *tensors)
+            got = make(handle, *tensors)
+            with _keeping:
+                if self.__dict__.get("_kept") is kept:
+                    if len(kept) >= 64:
+                        kept.clear()
+                    kept[key] = got
+                    plans = [p for p in (getattr(g, "plan", None) for g in kept.values()) if p is not None]
+                    self.__dict__["_plans"] = plans[::-1]  # the newest comes first
         return got
 
     def _prepare(self, h, *tensors):
-        """Checks a call and keeps it for _calls.run; the newest comes first."""
-        desc, specs, relaid = got = self._describe(h, *tensors)
+        """Checks a call and makes its plan for _calls.run."""
+        desc, specs, relaid = self._describe(h, *tensors)
         if _calls is None or relaid:
-            return got
+            return _Kept(desc, specs, relaid, None)
         present = [i for i, spec in enumerate(specs) if spec is not None]
         slots = tuple((s if tensors[s] is not None else None) if s >= 0 else
                       (-1 - present.index(-1 - s) if specs[-1 - s] is not None else None) for s in self.slots)
-        if self._plans is None:
-            self.__dict__["_plans"] = []
-        plan = _calls.Plan(_address(getattr(C.lib(), self.entry)), _address(C.lib().onnxb200_get_stream),
-                           ctypes.addressof(desc), desc, h.device, tensors, tuple(specs[i] for i in present), slots)
-        self._plans.insert(0, plan)
-        return got
+        return _Kept(desc, specs, relaid, _calls.Plan(
+            _address(getattr(C.lib(), self.entry)), _address(C.lib().onnxb200_get_stream), ctypes.addressof(desc), desc,
+            h.device, tensors, tuple(specs[i] for i in present), slots))
 
 
 class RMSNormalization(_Described, Operator):

@@ -260,3 +260,94 @@ def test_scales_side_by_side_at_the_edge(C):
     for row, block in ((2, 1), (1, 4), (3, 1), (1, 5), (1 << 37, 1 << 36), (1 << 35, 1 << 37)):
         assert call_norm(C, norm_desc(C, out_type=E4M3, y_scale_row=row, y_scale_block=block)) == C.ERR_INVALID_ARGUMENT
         assert call_quant(C, quant_desc(C, scale_row=row, scale_block=block)) == C.ERR_INVALID_ARGUMENT
+
+
+@pytest.fixture
+def kept_op(ob, monkeypatch):
+    """An operator that keeps its calls, with plans that only name the settings they were made under;
+    on_plan is called while a plan is made."""
+    import types
+
+    class Op(ob.ops._Described, ob.ops.Operator):
+        entry, slots, setting, on_plan = "onnxb200_quantize_blocks", (0, -1, -1), 0, None
+
+        def _settings(self):
+            return self.setting
+
+        def _describe(self, h, x):
+            return ob._capi.QuantizeDesc(rows=self.setting), (((2,), (1,), torch.float32),), ()
+
+        def see(self, size):
+            return self._described(types.SimpleNamespace(device=0), self._prepare, torch.zeros(size))
+
+    op = Op()
+
+    def plan(entry, get_stream, address, desc, device, tensors, outputs, slots):
+        if Op.on_plan:
+            Op.on_plan()
+        return types.SimpleNamespace(setting=desc.rows, size=tensors[0].numel())
+
+    monkeypatch.setattr(ob.ops, "_calls", types.SimpleNamespace(Plan=plan))
+    return op
+
+
+def test_settings_changed_while_a_call_is_described(kept_op):
+    """As by another thread: the call goes through, and nothing made under the old settings is kept."""
+    def change():
+        type(kept_op).on_plan = None
+        kept_op.setting = 5
+
+    type(kept_op).on_plan = staticmethod(change)
+    assert kept_op.see(3).plan.setting == 0
+    assert not kept_op._plans
+    assert kept_op.see(3).plan.setting == 5
+    assert [p.setting for p in kept_op._plans] == [5]
+
+
+def test_layouts_dropped_while_a_call_is_described(kept_op):
+    """Another thread sees so many layouts in the meantime that the oldest are dropped."""
+    def others():
+        type(kept_op).on_plan = None
+        for i in range(64):
+            kept_op.see(100 + i)
+
+    type(kept_op).on_plan = staticmethod(others)
+    assert kept_op.see(3).plan.size == 3
+    assert kept_op._plans[0].size == 3 and len(kept_op._plans) <= 64
+
+
+def test_operator_shared_by_threads(kept_op):
+    """Layouts and settings seen by several threads at once: no call fails, and every plan that is kept
+    was made under the settings of now."""
+    import sys
+    import threading
+    errors, stop = [], threading.Event()
+
+    def see(seed):
+        try:
+            i = 0
+            while not stop.is_set():
+                i += 1
+                got = kept_op.see(1 + (seed * 31 + i) % 97)
+                plans = kept_op._plans
+                assert got.plan is not None and (plans is None or len({p.setting for p in plans}) <= 1)
+        except Exception as e:  # noqa: BLE001 -- handed to the test's thread
+            errors.append(e)
+
+    was = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    threads = [threading.Thread(target=see, args=(i,)) for i in range(4)]
+    try:
+        for t in threads:
+            t.start()
+        for i in range(300):
+            kept_op.setting = i
+    finally:
+        stop.set()
+        for t in threads:
+            t.join()
+        sys.setswitchinterval(was)
+    assert not errors, errors[0]
+    for i in range(3):
+        kept_op.see(i)
+    assert all(p.setting == 299 for p in kept_op._plans)
