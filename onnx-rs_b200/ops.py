@@ -693,7 +693,7 @@ class _Described:
             with _keeping:
                 if self.__dict__.get("_kept") is kept:
                     if len(kept) >= 64:
-                        kept.clear()
+                        del kept[next(iter(kept))]  # the oldest
                     kept[key] = got
                     plans = [p for p in (getattr(g, "plan", None) for g in kept.values()) if p is not None]
                     self.__dict__["_plans"] = plans[::-1]  # the newest comes first

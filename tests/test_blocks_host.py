@@ -351,3 +351,13 @@ def test_operator_shared_by_threads(kept_op):
     for i in range(3):
         kept_op.see(i)
     assert all(p.setting == 299 for p in kept_op._plans)
+
+
+def test_the_oldest_layout_is_dropped(kept_op):
+    """A call with a 65th layout takes the place of the first: the others stay as they were kept."""
+    first = [kept_op.see(i) for i in range(64)]
+    kept_op.see(64)
+    assert len(kept_op._kept) == 64
+    assert [p.size for p in kept_op._plans] == list(range(64, 0, -1))
+    assert all(kept_op.see(i) is first[i] for i in range(1, 64))
+    assert kept_op.see(0) is not first[0]
