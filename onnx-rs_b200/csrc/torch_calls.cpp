@@ -10,7 +10,9 @@
 //
 // A Plan holds no tensor and no address of one.  What it cannot serve (other
 // layouts, another current device, a handle on another stream than torch's)
-// run() answers with None, and the operator goes the long way.
+// run() answers with None, and the operator goes the long way.  The module belongs to
+// the Python and torch that it was built with (CALLS_PYTHON, CALLS_TORCH): another
+// Python cannot import it, for another torch the operators leave it alone.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
@@ -20,6 +22,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstring>
 #include <vector>
 
 namespace {
@@ -216,7 +219,22 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods};
 
 }  // namespace
 
+#define CALLS_TEXT_OF(x) #x
+#define CALLS_TEXT(x) CALLS_TEXT_OF(x)
+
+// The version that Python reports begins with `built`, its major and minor numbers.
+static bool same_python(const char* built) {
+  const size_t n = strlen(built);
+  const char* v = Py_GetVersion();
+  return strncmp(v, built, n) == 0 && (v[n] < '0' || v[n] > '9');
+}
+
 PyMODINIT_FUNC PyInit__calls() {
+  // before anything whose layout belongs to a version of Python
+  if (!same_python(CALLS_TEXT(CALLS_PYTHON))) {
+    PyErr_SetString(PyExc_ImportError, "built for Python " CALLS_TEXT(CALLS_PYTHON));
+    return nullptr;
+  }
   plan_type.tp_name = "_calls.Plan";
   plan_type.tp_basicsize = sizeof(Plan);
   plan_type.tp_flags = Py_TPFLAGS_DEFAULT;
@@ -225,7 +243,8 @@ PyMODINIT_FUNC PyInit__calls() {
   if (PyType_Ready(&plan_type) < 0) return nullptr;
   PyObject* m = PyModule_Create(&module);
   if (!m) return nullptr;
-  if (PyModule_AddObjectRef(m, "Plan", reinterpret_cast<PyObject*>(&plan_type)) < 0) {
+  if (PyModule_AddObjectRef(m, "Plan", reinterpret_cast<PyObject*>(&plan_type)) < 0 ||
+      PyModule_AddStringConstant(m, "torch_version", CALLS_TEXT(CALLS_TORCH)) < 0) {
     Py_DECREF(m);
     return nullptr;
   }

@@ -16,9 +16,11 @@ character codes instead, src/ops/registry.rs:105-106, and never matches).
 from __future__ import annotations
 
 import ctypes
+import importlib
 import math
 import os
 import threading
+import warnings
 from typing import Dict, List, NamedTuple, Optional, Sequence
 
 import torch
@@ -26,10 +28,33 @@ import torch
 from . import _capi as C
 from .runtime import (Handle, InvalidOperator, UnsupportedFeature, ValidationError, dptr)
 
-# the native module for repeated calls (make -C csrc calls); ctypes does without it
-_calls = None
-if os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "_calls.so")):
-    from . import _calls
+
+def _load_calls():
+    """The native module for repeated calls (make -C csrc calls), or None: ctypes does without it."""
+    if not os.path.exists(os.path.join(os.path.dirname(os.path.abspath(__file__)), "_calls.so")):
+        return None
+    try:
+        module = importlib.import_module("._calls", __package__)
+        built_for = getattr(module, "torch_version", "of an unknown version")
+        if built_for != torch.__version__:
+            raise ImportError(f"built for torch {built_for}, not {torch.__version__}")
+        return module
+    except ImportError as e:
+        warnings.warn(f"onnx-rs_b200/_calls.so is not used ({e}); calls go through ctypes", RuntimeWarning, stacklevel=2)
+        return None
+
+
+def _native():
+    """ops._calls, loaded where it is asked for first: importing the package does not need it."""
+    if "_calls" not in globals():
+        globals()["_calls"] = _load_calls()
+    return _calls
+
+
+def __getattr__(name):
+    if name == "_calls":
+        return _native()
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class ExecutionContext:
@@ -670,7 +695,7 @@ class _Described:
     def _call(self, h, *tensors):
         plans = self._plans
         if plans:
-            out = _calls.run(plans, h.address, h.device, h.own_stream_ptr, *tensors)
+            out = _native().run(plans, h.address, h.device, h.own_stream_ptr, *tensors)
             if type(out) is list:
                 return out
             if out is not None:
@@ -702,12 +727,12 @@ class _Described:
     def _prepare(self, h, *tensors):
         """Checks a call and makes its plan for _calls.run."""
         desc, specs, relaid = self._describe(h, *tensors)
-        if _calls is None or relaid:
+        if relaid or _native() is None:
             return _Kept(desc, specs, relaid, None)
         present = [i for i, spec in enumerate(specs) if spec is not None]
         slots = tuple((s if tensors[s] is not None else None) if s >= 0 else
                       (-1 - present.index(-1 - s) if specs[-1 - s] is not None else None) for s in self.slots)
-        return _Kept(desc, specs, relaid, _calls.Plan(
+        return _Kept(desc, specs, relaid, _native().Plan(
             _address(getattr(C.lib(), self.entry)), _address(C.lib().onnxb200_get_stream), ctypes.addressof(desc), desc,
             h.device, tensors, tuple(specs[i] for i in present), slots))
 
