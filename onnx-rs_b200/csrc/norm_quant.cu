@@ -179,11 +179,22 @@ __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, CH == 4 && 
   Vec8<W> vw[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) vw[c].load(static_cast<const W*>(p.weight) + at(c) * 8, at(c) < n8);
-  float ss = 0.f;
+  // A sum per vector, then pairs: 8 + log2(CH) + 5 roundings lie on the way of a square
+  // (and 5 over the warps of a block), where one sum per thread has up to 32 + 5 and was
+  // wrong by as much for a row of one large element and many small ones.
+  float ss, sq[CH];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    sq[c] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(h[c][j], h[c][j], ss);
+    for (int j = 0; j < 8; ++j) sq[c] = fmaf(h[c][j], h[c][j], sq[c]);
+  }
+  if constexpr (CH == 4)
+    ss = (sq[0] + sq[1]) + (sq[2] + sq[3]);
+  else if constexpr (CH == 2)
+    ss = sq[0] + sq[1];
+  else
+    ss = sq[0];
   ss = warp_sum(ss);
   if (!WARP && (threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
   if (p.sum) {
