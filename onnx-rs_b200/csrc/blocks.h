@@ -59,6 +59,16 @@ constexpr int64_t matmul_vec_smem(int m, int k) {
   return m * (((int64_t)k + 15) / 16 * 32 + ((int64_t)k + kQBlock - 1) / kQBlock * 4);
 }
 constexpr bool matmul_takes_vec(int m, int k) { return m <= 2 && matmul_vec_smem(m, k) <= kVecMaxSmem; }
+// Many rows: tiles of 256 x 256 or 256 x 128 on num_sms / 2 pairs of thread blocks.  A
+// wave of the narrow ones takes ~0.6 of a wave of the wide ones (8.5 and 16 us at k =
+// 4096; 200 x 8192: 15.3 and 20.4 us, 512 x 8192: 23.4 and 21.4 us, 4096 x 4096: 70.6 and
+// 67.2 us).
+constexpr bool matmul_takes_wide(int m, int n, int num_sms) {
+  const int64_t tm = ((int64_t)m + 255) / 256, pairs = num_sms / 2;
+  const int64_t wide = (tm * (((int64_t)n + 255) / 256) + pairs - 1) / pairs;
+  const int64_t narrow = (tm * (((int64_t)n + 127) / 128) + pairs - 1) / pairs;
+  return 3 * narrow >= 5 * wide;
+}
 int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t stream);
 
 }  // namespace ob2

@@ -1030,11 +1030,7 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
     // split k eight ways (64 x 4096 x 4096: 10.7 us, 12.5 on pairs; with 64 tiles of
     // columns, 64 x 8192 x 4096, 18.7 and 15.4).
     if (a.m > 64 || (a.m > 32 && (a.n + 127) / 128 * 4 > num_sms)) {
-      // Tiles of 256 x 256 or 256 x 128 on num_sms / 2 pairs: a wave of the narrow
-      // ones takes ~0.6 of a wave of the wide ones (8.5 and 16 us at k = 4096; 200 x
-      // 8192: 15.3 and 20.4 us, 512 x 8192: 23.4 and 21.4 us, 4096 x 4096: 70.6 and 67.2 us).
       const int64_t tm = (a.m + 255) / 256, pairs = num_sms / 2;
-      const int64_t wide = (tm * ((a.n + 255) / 256) + pairs - 1) / pairs, narrow = (tm * ((a.n + 127) / 128) + pairs - 1) / pairs;
       // Few tiles: two or four pairs share one, where all run at once (with one, two and
       // four: 256 x 1024 x 4096 13.2, 12.3 and 10.6 us; 100 x 1000 x 14336 30.9, 21.6 and
       // 15.5; but 200 x 2048 x 4096, whose 16 clusters of eight CTAs take two turns, 13.3,
@@ -1047,7 +1043,7 @@ int matmul_blocks_launch(const MatmulBlocksArgs& a, int num_sms, cudaStream_t st
       };
       if (tiles * 4 <= pairs && kbs >= 16 && tiles <= at_once(4)) return launch_pair<T, 128, true>(a, num_sms, st, 4);
       if (tiles * 2 <= pairs && kbs >= 28 && tiles <= at_once(2)) return launch_pair<T, 128, true>(a, num_sms, st, 2);
-      return 3 * narrow < 5 * wide ? launch_pair<T, 128>(a, num_sms, st) : launch_pair<T, 256>(a, num_sms, st);
+      return matmul_takes_wide(a.m, a.n, num_sms) ? launch_pair<T, 256>(a, num_sms, st) : launch_pair<T, 128>(a, num_sms, st);
     }
     if (matmul_takes_vec(a.m, a.k)) return a.m == 1 ? launch_vec<T, 1>(a, st) : launch_vec<T, 2>(a, st);
     return a.m <= 16   ? launch_rows<T, 16>(a, rows_split<T, 16>(a, num_sms), st)

@@ -42,3 +42,18 @@ def test_shared_memory_of_the_product_for_one_or_two_rows(tmp_path):
     for m, k, smem, takes in got:
         assert smem == m * (-(-k // 16) * 32 + -(-k // 128) * 4)
         assert takes == (m <= 2 and smem <= 100 * 1024)
+
+
+# Products with several tiles for a pair of thread blocks, on the 148 SMs of a B200: (m, n, whether tiles are 256 wide)
+TILED = [(1777, 5000, True), (2300, 4700, True), (1800, 5003, True), (4096, 4096, True), (8192, 8192, True), (1500, 6700, True),
+         (700, 6400, False), (600, 6404, False), (200, 8192, False), (256, 512, False), (1500, 777, False), (70000, 300, False)]
+
+
+def test_tile_width_of_products_with_many_rows(tmp_path):
+    """Wide tiles where their waves take no longer: a wave of narrow ones takes 0.6 of theirs."""
+    got = run_cpp(tmp_path, "const int mn[][2] = {%s};\nfor (auto& v : mn) printf(\"%%d %%d %%d\\n\", v[0], v[1], "
+                  "(int)matmul_takes_wide(v[0], v[1], 148));" % ", ".join("{%d, %d}" % t[:2] for t in TILED))
+    assert [(m, n, bool(w)) for m, n, w in got] == TILED
+    for m, n, wide in got:
+        waves = [-(-(-(-m // 256) * -(-n // bn)) // 74) for bn in (128, 256)]
+        assert wide == (3 * waves[0] >= 5 * waves[1])
