@@ -850,21 +850,29 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         const int col = nt * BN + c;
         if (row < p.m && col < p.n) {
-          T e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if (p.bias) v[j] += p.bias[min(col + j, p.n - 1)];
             if (p.relu) v[j] = v[j] < 0.f ? 0.f : v[j];  // NaN stays NaN
-            e[j] = from_f32<T>(v[j]);
           }
           T* dst = static_cast<T*>(p.y) + row * p.ldy + col;
           if (vec && col + 8 <= p.n) {
 #pragma unroll
-            for (int u = 0; u < 8 / PER; ++u) reinterpret_cast<uint4*>(dst)[u] = reinterpret_cast<const uint4*>(e)[u];
+            for (int u = 0; u < 8 / PER; ++u) {
+              uint32_t w[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if constexpr (sizeof(T) == 4)
+                  w[q] = __float_as_uint(v[u * 4 + q]);
+                else
+                  w[q] = pack_rounded<T>(v[2 * q], v[2 * q + 1]);
+              }
+              reinterpret_cast<uint4*>(dst)[u] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              if (col + j < p.n) dst[j] = e[j];
+              if (col + j < p.n) dst[j] = from_f32<T>(v[j]);
           }
         }
       }

@@ -134,3 +134,20 @@ def test_product_with_many_tiles_nan_stays_in_its_row_and_column(ob, ctx, m, n):
             y[row], want[row] = 0, 0
             y[:, col], want[:, col] = 0, 0
             assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n,k", [(256, 512, 2560), (100, 1000, 2048), (200, 1004, 3700), (129, 2565, 3700)])
+def test_product_with_shared_tiles(handle, m, n, k, t):
+    """Tiles shared by two or four pairs of thread blocks, in every type: 16 bytes of y at a time where its
+    rows are on the grid, the last columns and other rows by elements, and nothing beside them."""
+    a, sa, b, sb = tb.operands(m, n, k, m + n)
+    bias = tb.normal((n,), 3)
+    for off, width in ((8, n + 24 - n % 8), (1, n + 24 - n % 8), (0, n + 1)):
+        y = torch.full((m + 2, width), 3.0, dtype=t, device="cuda")
+        inner = y[1:-1, off:off + n]
+        tb.run_mm(handle, a, sa, b, sb, bias, inner, relu=True)
+        check_mm(inner, a, sa, b, sb, bias, True, t)
+        rest = y.clone()
+        rest[1:-1, off:off + n] = 3.0
+        assert (rest == 3.0).all()
