@@ -296,7 +296,7 @@ typedef struct onnxb200_rmsnorm_desc {
   int64_t y_scale_row, y_scale_block;  /* strides of y_scale (out_type E4M3) */
   int type;                            /* of x, residual and sum: F32, F16 or BF16 */
   int weight_type;                     /* F32, F16 or BF16 */
-  int out_type;                        /* of y: the same as `type`, or E4M3 */
+  int out_type;                        /* of y: `type`, `weight_type` (ONNX's Y) or E4M3 */
   float epsilon;                       /* >= 0 */
 } onnxb200_rmsnorm_desc;
 /* ONNX RMSNormalization (opset 23) over the last axis, with the addition in

@@ -78,7 +78,8 @@ extern "C" {
 int onnxb200_rmsnorm(onnxb200_handle* h, const onnxb200_rmsnorm_desc* d, const void* x, const void* residual,
                      const void* weight, void* sum, void* y, float* y_scale) {
   if (!d) return fail(h, ONNXB200_ERR_INVALID_ARGUMENT, "RMSNormalization: null descriptor");
-  if (!wide_type(d->type) || !wide_type(d->weight_type) || (d->out_type != d->type && d->out_type != kE4M3))
+  if (!wide_type(d->type) || !wide_type(d->weight_type) ||
+      (d->out_type != d->type && d->out_type != d->weight_type && d->out_type != kE4M3))
     return fail(h, ONNXB200_ERR_VALIDATION, "RMSNormalization: unsupported element type");
   if (d->rows < 0 || d->rows > kMaxDim || d->cols <= 0)
     return fail(h, ONNXB200_ERR_VALIDATION, "RMSNormalization: invalid shape");

@@ -84,6 +84,15 @@ struct Vec8 {
   }
 };
 
+// f(row r of y) in y's type: x's, or the weight's.
+template <typename T, typename W, typename F>
+__device__ __forceinline__ void with_out(const RmsNormArgs& p, int64_t r, F f) {
+  if (std::is_same_v<T, W> || p.out_type == p.type)
+    f(static_cast<T*>(p.y) + r * p.ldy);
+  else
+    f(static_cast<W*>(p.y) + r * p.ldy);
+}
+
 // Eight values times inv, in e4m3.
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[8], float inv) {
   *reinterpret_cast<uint2*>(p) = make_uint2(to_e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
@@ -221,13 +230,14 @@ __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, CH == 4 && 
     for (int j = 0; j < 8; ++j) h[c][j] = h[c][j] * rstd * f[j];
   }
   if (p.out_type != kE4M3) {
-    T* y = static_cast<T*>(p.y) + r * p.ldy;
+    with_out<T, W>(p, r, [&](auto* y) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      Vec8<T> o;
-      o.pack(h[c]);
-      if (at(c) < n8) o.store(y + at(c) * 8);
-    }
+      for (int c = 0; c < CH; ++c) {
+        Vec8<std::remove_pointer_t<decltype(y)>> o;
+        o.pack(h[c]);
+        if (at(c) < n8) o.store(y + at(c) * 8);
+      }
+    });
     return;
   }
 #pragma unroll
@@ -321,12 +331,13 @@ __global__ void __launch_bounds__(kRowThreads, NB == 1 ? 4 : 2) rmsnorm_elem_ker
     }
   }
   if (p.out_type != kE4M3) {
-    T* y = static_cast<T*>(p.y) + r * p.ldy;
+    with_out<T, W>(p, r, [&](auto* y) {
 #pragma unroll
-    for (int c = 0; c < NB; ++c)
+      for (int c = 0; c < NB; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (at(c, j) < p.cols) y[at(c, j)] = from_f32<T>(h[c][j]);
+        for (int j = 0; j < 4; ++j)
+          if (at(c, j) < p.cols) y[at(c, j)] = from_f32<std::remove_pointer_t<decltype(y)>>(h[c][j]);
+    });
     return;
   }
   uint8_t* q = static_cast<uint8_t*>(p.y) + r * p.ldy;
@@ -381,8 +392,10 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_row_kernel(const RmsNormA
   for (int i = 0; i < kRowThreads / 32; ++i) tot += part[i];
   const float rstd = 1.f / sqrtf(tot / (float)p.cols + p.eps);
   if (p.out_type != kE4M3) {
-    T* y = static_cast<T*>(p.y) + r * p.ldy;
-    for (int i = threadIdx.x; i < p.cols; i += kRowThreads) y[i] = from_f32<T>(row[i] * rstd * to_f32(w[i]));
+    with_out<T, W>(p, r, [&](auto* y) {
+      for (int i = threadIdx.x; i < p.cols; i += kRowThreads)
+        y[i] = from_f32<std::remove_pointer_t<decltype(y)>>(row[i] * rstd * to_f32(w[i]));
+    });
     return;
   }
   uint8_t* q = static_cast<uint8_t*>(p.y) + r * p.ldy;
@@ -583,7 +596,7 @@ int rmsnorm_launch(const RmsNormArgs& a, int num_sms, cudaStream_t st) {
       const bool quant = a.out_type == kE4M3;
       const bool vec = a.cols % 8 == 0 && a.cols <= 4 * 512 * 8 && on_grid(a.x, a.ldx, sizeof(T), 16) &&
                        (!a.res || on_grid(a.res, a.ldr, sizeof(T), 16)) && (!a.sum || on_grid(a.sum, a.lds, sizeof(T), 16)) &&
-                       on_grid(a.weight, 0, sizeof(W), 16) && on_grid(a.y, a.ldy, quant ? 1 : sizeof(T), quant ? 8 : 16);
+                       on_grid(a.weight, 0, sizeof(W), 16) && on_grid(a.y, a.ldy, elem_size(a.out_type), quant ? 8 : 16);
       // Short rows off the grid stay in registers, a warp for one or two blocks of columns
       // (4096 x 1001 fp16: 13.7 us, 22.6 in shared memory; 4096 x 3001 bf16 28.4 and 30.0);
       // with four a warp the registers left too few warps (8192 x 8001: 167 us and 138).

@@ -743,24 +743,29 @@ class RMSNormalization(_Described, Operator):
     compute([x, scale], ctx, residual=None) returns [y], or with ``quantize`` [q, q_scale]: e4m3
     values and one fp32 scale for every 128 columns of a row, the operand form of
     MatMulBlockScaled.  With a residual, h = x + residual is normalised and h (rounded to x's
-    type) is returned as the last output."""
+    type) is returned as the last output.  Where x and scale differ in type, y has x's, or with
+    ``y_like="scale"`` the scale's: so ONNX defines it, and so operators made from nodes do."""
     op_type = "RMSNormalization"
     min_inputs = 2
     entry = "onnxb200_rmsnorm"
     slots = (0, 2, 1, -3, -1, -2)  # x, residual, scale; h, y, y_scale
 
-    def __init__(self, epsilon=1e-5, axis=-1, quantize=False):
+    def __init__(self, epsilon=1e-5, axis=-1, quantize=False, y_like="x"):
+        if y_like not in ("x", "scale"):
+            raise ValidationError(C.ERR_VALIDATION, f"RMSNormalization: y_like must be 'x' or 'scale', got {y_like!r}")
         self.epsilon = float(epsilon)
         self.axis = int(axis)
         self.quantize = bool(quantize)
+        self.y_like = y_like
 
     @classmethod
     def from_node(cls, node, **kw):
         a = _attrs(node)
+        kw.setdefault("y_like", "scale")
         return cls(a.get("epsilon", 1e-5), a.get("axis", -1), **kw)
 
     def _settings(self):
-        return self.epsilon, self.axis, self.quantize
+        return self.epsilon, self.axis, self.quantize, self.y_like
 
     def _check_axis(self, rank):
         if self.axis not in (-1, rank - 1):
@@ -790,15 +795,16 @@ class RMSNormalization(_Described, Operator):
         rows = math.prod(lead)
         d.rows, d.cols = rows, cols
         d.epsilon = self.epsilon
-        d.out_type = d.type
+        y = x if self.y_like == "x" else w
+        d.out_type = d.type if y is x else d.weight_type
         if self.quantize:
             d.out_type = C.TYPE_E4M3
             d.ldy = _stored_stride(cols)
             d.y_scale_row, d.y_scale_block = 1, max(1, rows)
         blocks = (cols + _QBLOCK - 1) // _QBLOCK
-        same = _dense(x.shape, x.dtype)
-        return d, (_stored_rows(lead, cols) if self.quantize else same,
-                   _stored_scales(lead, rows, blocks) if self.quantize else None, same if residual is not None else None), ()
+        return d, (_stored_rows(lead, cols) if self.quantize else _dense(x.shape, y.dtype),
+                   _stored_scales(lead, rows, blocks) if self.quantize else None,
+                   _dense(x.shape, x.dtype) if residual is not None else None), ()
 
     def compute(self, inputs, ctx, residual=None):
         return self._call(ctx.handle, inputs[0], inputs[1], residual)

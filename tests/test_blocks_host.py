@@ -361,3 +361,17 @@ def test_the_oldest_layout_is_dropped(kept_op):
     assert [p.size for p in kept_op._plans] == list(range(64, 0, -1))
     assert all(kept_op.see(i) is first[i] for i in range(1, 64))
     assert kept_op.see(0) is not first[0]
+
+
+def test_norm_output_in_the_type_of_the_weight(ob, C):
+    """ONNX gives y the scale's type: taken by the entry, and what operators made from nodes ask for."""
+    assert call_norm(C, norm_desc(C, weight_type=F32, out_type=F32)) == C.ERR_INVALID_ARGUMENT
+    assert call_norm(C, norm_desc(C, weight_type=F16, out_type=F16)) == C.ERR_INVALID_ARGUMENT
+    assert call_norm(C, norm_desc(C, weight_type=F32, out_type=F16)) == C.ERR_VALIDATION
+    assert call_norm(C, norm_desc(C, weight_type=F32, out_type=F32), y=ctypes.c_void_p(4098)) == C.ERR_VALIDATION
+    node = {"op": "RMSNormalization", "inputs": ["x", "w"], "outputs": ["y"], "attrs": {}}
+    r = ob.OperatorRegistry.initialize_standard_operators()
+    assert r.create_operator_for_node(node, opset=23).y_like == "scale"
+    assert ob.RMSNormalization().y_like == ob.RMSNormalization.from_node(node, y_like="x").y_like == "x"
+    with pytest.raises(ob.ValidationError):
+        ob.RMSNormalization(y_like="residual")

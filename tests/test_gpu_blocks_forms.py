@@ -151,3 +151,41 @@ def test_product_with_shared_tiles(handle, m, n, k, t):
         rest = y.clone()
         rest[1:-1, off:off + n] = 3.0
         assert (rest == 3.0).all()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("wt", TYPES)
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 256), (400, 256), (400, 1000), (300, 2056), (2, 4096), (3, 1001), (3, 3001), (3, 6001),
+                                       (2, 20000)])
+def test_norm_of_a_node_has_the_type_of_its_scale(ob, ctx, rows, cols, t, wt, residual):
+    """As ONNX defines it: y in the scale's type, rounded once; x + residual stays in x's.  The longest chain
+    of roundings is a row's of 20000 columns in shared memory: a square's and 40 additions in a thread, 5 over
+    its warp, 16 over the warps, of which the root passes half, and 7 as on the grid: 38 u."""
+    node = {"op": "RMSNormalization", "inputs": ["x", "w"], "outputs": ["y"], "attrs": {"epsilon": 1e-5}}
+    op = ob.OperatorRegistry.initialize_standard_operators().create_operator_for_node(node, opset=23)
+    x = tb.normal((rows, cols), rows + cols, t)
+    r = 3 * tb.normal((rows, cols), 7, t) if residual else None
+    w = (1 + 0.3 * tb.normal((cols,), 9)).to(wt)
+    out = op.compute([x, w], ctx, residual=r)
+    h, y = tb.norm_ref(x, r, w, 1e-5)
+    assert out[0].dtype == wt and out[0].shape == x.shape
+    slack = 38 * U * (1 + 2 ** -10)
+    assert ((out[0].double() - y).abs() <= y.abs() * (tb.half(wt) + slack) * (1 + tb.half(wt)) + tb.TINY[wt]).all()
+    if residual:
+        assert out[1].dtype == t and ((out[1].double() - h).abs() <= h.abs() * (tb.half(t) + U) * (1 + U) + tb.TINY[t]).all()
+
+
+@pytest.mark.parametrize("cols", [256, 1001, 6001])
+def test_norm_into_the_type_of_the_weight_writes_nothing_else(handle, cols):
+    """fp32 rows of y inside a larger matrix, x in bf16."""
+    x, w = tb.normal((5, cols), 1, torch.bfloat16), tb.normal((cols,), 2)
+    for off in (4, 1):
+        y = torch.full((7, cols + 16 - cols % 8), 3.0, device="cuda")
+        inner = y[1:-1, off:off + cols]
+        tb.run_norm(handle, x, None, w, None, inner, None)
+        ref = tb.norm_ref(x, None, w, 1e-5)[1]
+        assert ((inner.double() - ref).abs() <= ref.abs() * 39 * U * (1 + 2 ** -10)).all()
+        rest = y.clone()
+        rest[1:-1, off:off + cols] = 3.0
+        assert (rest == 3.0).all()
