@@ -761,6 +761,9 @@ class RMSNormalization(_Described, Operator):
     @classmethod
     def from_node(cls, node, **kw):
         a = _attrs(node)
+        if a.get("stash_type", 1) != 1:
+            raise UnsupportedFeature(C.ERR_UNSUPPORTED,
+                                     f"RMSNormalization: computes in float32 (stash_type 1), got stash_type {a['stash_type']}")
         kw.setdefault("y_like", "scale")
         return cls(a.get("epsilon", 1e-5), a.get("axis", -1), **kw)
 

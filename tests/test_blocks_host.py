@@ -375,3 +375,13 @@ def test_norm_output_in_the_type_of_the_weight(ob, C):
     assert ob.RMSNormalization().y_like == ob.RMSNormalization.from_node(node, y_like="x").y_like == "x"
     with pytest.raises(ob.ValidationError):
         ob.RMSNormalization(y_like="residual")
+
+
+def test_norm_refuses_other_stash_types(ob):
+    """Sums are fp32: a node that asks for another type of its intermediate values is not silently taken."""
+    node = {"op": "RMSNormalization", "inputs": ["x", "w"], "outputs": ["y"], "attrs": {"stash_type": 1}}
+    assert ob.RMSNormalization.from_node(node).epsilon == 1e-5
+    for t in (10, 11, 16):
+        node["attrs"]["stash_type"] = t
+        with pytest.raises(ob.UnsupportedFeature):
+            ob.RMSNormalization.from_node(node)
