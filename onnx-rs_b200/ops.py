@@ -833,11 +833,17 @@ class QuantizeBlocks(_Described, Operator):
     def from_node(cls, node, **kw):
         return cls(_attrs(node).get("block_rows", 1), **kw)
 
+    @staticmethod
+    def _check_rank(block_rows, rank):
+        if rank == 0 or (block_rows != 1 and rank != 2):
+            raise ValidationError(C.ERR_VALIDATION, "QuantizeBlocks: " + ("weights must be 2-D" if rank else "expected at least one dimension"))
+
     def output_shapes(self, node, input_shapes):
         x = input_shapes[0]
         if x is None:
             return [None, None]
         br = type(self).from_node(node).block_rows
+        self._check_rank(br, len(x))
         blocks = (x[-1] + _QBLOCK - 1) // _QBLOCK
         return [list(x), list(x[:-1]) + [blocks] if br == 1 else [(x[0] + _QBLOCK - 1) // _QBLOCK, blocks]]
 
@@ -847,8 +853,7 @@ class QuantizeBlocks(_Described, Operator):
         d = C.QuantizeDesc()
         d.type = _type(x, what)
         d.ldx = _row_stride(x, what)
-        if self.block_rows != 1 and x.dim() != 2:
-            raise ValidationError(C.ERR_VALIDATION, f"{what}: weights must be 2-D")
+        self._check_rank(self.block_rows, x.dim())
         lead, cols = tuple(x.shape[:-1]), x.shape[-1]
         rows, blocks = math.prod(lead), (cols + _QBLOCK - 1) // _QBLOCK
         d.rows, d.cols, d.ldq = rows, cols, _stored_stride(cols)

@@ -385,3 +385,17 @@ def test_norm_refuses_other_stash_types(ob):
         node["attrs"]["stash_type"] = t
         with pytest.raises(ob.UnsupportedFeature):
             ob.RMSNormalization.from_node(node)
+
+
+def test_quantize_shapes_are_refused_as_the_call_is(ob):
+    """Weights are 2-D, activations have a last axis: shape inference says so before a call does."""
+    node = {"op": "QuantizeBlocks", "inputs": ["x"], "outputs": ["q", "s"], "attrs": {"block_rows": 128}}
+    op = ob.QuantizeBlocks(128)
+    for shape in ([300], [4, 300, 130], []):
+        with pytest.raises(ob.ValidationError):
+            op.output_shapes(node, [shape])
+    assert op.output_shapes(node, [None]) == [None, None]
+    node["attrs"] = {}
+    assert ob.QuantizeBlocks().output_shapes(node, [[300]]) == [[300], [3]]
+    with pytest.raises(ob.ValidationError):
+        ob.QuantizeBlocks().output_shapes(node, [[]])
