@@ -751,8 +751,7 @@ class RMSNormalization(_Described, Operator):
     slots = (0, 2, 1, -3, -1, -2)  # x, residual, scale; h, y, y_scale
 
     def __init__(self, epsilon=1e-5, axis=-1, quantize=False, y_like="x"):
-        if y_like not in ("x", "scale"):
-            raise ValidationError(C.ERR_VALIDATION, f"RMSNormalization: y_like must be 'x' or 'scale', got {y_like!r}")
+        self._check_y_like(y_like)
         self.epsilon = float(epsilon)
         self.axis = int(axis)
         self.quantize = bool(quantize)
@@ -769,6 +768,11 @@ class RMSNormalization(_Described, Operator):
 
     def _settings(self):
         return self.epsilon, self.axis, self.quantize, self.y_like
+
+    @staticmethod
+    def _check_y_like(y_like):
+        if y_like not in ("x", "scale"):
+            raise ValidationError(C.ERR_VALIDATION, f"RMSNormalization: y_like must be 'x' or 'scale', got {y_like!r}")
 
     def _check_axis(self, rank):
         if self.axis not in (-1, rank - 1):
@@ -798,6 +802,7 @@ class RMSNormalization(_Described, Operator):
         rows = math.prod(lead)
         d.rows, d.cols = rows, cols
         d.epsilon = self.epsilon
+        self._check_y_like(self.y_like)
         y = x if self.y_like == "x" else w
         d.out_type = d.type if y is x else d.weight_type
         if self.quantize:
@@ -880,11 +885,15 @@ class MatMulBlockScaled(_Described, Operator):
     slots = (0, 1, 2, 3, 4, -1)
 
     def __init__(self, dtype=torch.float32, relu=False):
+        self._check_dtype(dtype)
+        self.dtype = dtype
+        self.relu = bool(relu)
+
+    @staticmethod
+    def _check_dtype(dtype):
         if dtype not in _TYPE:
             raise ValidationError(C.ERR_VALIDATION,
                                   f"MatMulBlockScaled: expected float32, float16 or bfloat16, got {dtype}")
-        self.dtype = dtype
-        self.relu = bool(relu)
 
     def _settings(self):
         return self.dtype, self.relu
@@ -924,6 +933,7 @@ class MatMulBlockScaled(_Described, Operator):
             if t.data_ptr() != s.data_ptr():
                 relaid.append((i, lambda s, rows=rows: _scale_strides(s, rows, blocks, what)[0]))
         d.a_scale_row, d.a_scale_block, d.b_scale_row, d.b_scale_block = strides
+        self._check_dtype(self.dtype)
         d.out_type = _TYPE[self.dtype]
         d.flags = C.EPI_RELU if self.relu else 0
         return d, (_dense((*a.shape[:-1], n), self.dtype),), relaid

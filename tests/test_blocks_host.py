@@ -399,3 +399,20 @@ def test_quantize_shapes_are_refused_as_the_call_is(ob):
     assert ob.QuantizeBlocks().output_shapes(node, [[300]]) == [[300], [3]]
     with pytest.raises(ob.ValidationError):
         ob.QuantizeBlocks().output_shapes(node, [[]])
+
+
+def test_settings_changed_after_construction_are_checked(ob, monkeypatch):
+    """As the constructor checks them, at the next call."""
+    monkeypatch.setattr(ob.ops, "_check_device", lambda *a: None)
+    x, w = torch.zeros(4, 256), torch.ones(256)
+    norm = ob.RMSNormalization()
+    norm._describe(None, x, w, None)
+    norm.y_like = "weight"
+    with pytest.raises(ob.ValidationError):
+        norm._describe(None, x, w, None)
+    e4m3 = torch.zeros(4, 256).to(torch.float8_e4m3fn)
+    mm = ob.MatMulBlockScaled()
+    mm._describe(None, e4m3, torch.ones(4, 2), e4m3, torch.ones(1, 2), None)
+    mm.dtype = torch.float64
+    with pytest.raises(ob.ValidationError):
+        mm._describe(None, e4m3, torch.ones(4, 2), e4m3, torch.ones(1, 2), None)
