@@ -668,7 +668,9 @@ class _Kept(NamedTuple):
     plan: object     # of the native module, or None
 
 
-_keeping = threading.Lock()  # held to publish what operators keep, never during a call's own work
+# Held to publish what operators keep, never during a call's own work; a finaliser that the collector
+# runs meanwhile may change an operator's settings.
+_keeping = threading.RLock()
 
 
 class _Described:

@@ -416,3 +416,17 @@ def test_settings_changed_after_construction_are_checked(ob, monkeypatch):
     mm.dtype = torch.float64
     with pytest.raises(ob.ValidationError):
         mm._describe(None, e4m3, torch.ones(4, 2), e4m3, torch.ones(1, 2), None)
+
+
+def test_settings_changed_by_a_finaliser(ob, kept_op):
+    """The collector may run one wherever a list grows, so also while what is kept is published."""
+    import threading
+
+    def finalise():
+        with ob.ops._keeping:  # as a thread that publishes
+            kept_op.setting = 7
+
+    t = threading.Thread(target=finalise, daemon=True)
+    t.start()
+    t.join(10)
+    assert not t.is_alive() and kept_op.see(3).plan.setting == 7
