@@ -305,7 +305,10 @@ typedef struct onnxb200_rmsnorm_desc {
  *   y = h / sqrt(mean(h^2) + epsilon) * weight.
  * Everything between the loads and the stores is fp32: y is computed from the
  * unrounded h, and rounded (or quantised, with y_scale) once.  sum and y may be
- * the same memory as x or residual (same type and row stride). */
+ * the same memory as x or residual (same type and row stride).  The sum of h^2
+ * has fp32's range: a finite row where it passes 3.4e38 (one element of 1.9e19,
+ * or many smaller ones) gives zeros, and with epsilon 0 a row whose squares all
+ * vanish (elements below 2.6e-23) values that are not finite. */
 ONNXB200_API int onnxb200_rmsnorm(onnxb200_handle* h, const onnxb200_rmsnorm_desc* d, const void* x,
                                   const void* residual, const void* weight, void* sum, void* y,
                                   float* y_scale);
@@ -333,7 +336,8 @@ typedef struct onnxb200_matmul_blocks_desc {
  * sum_{k in j} a[m][k] * b[n][k], + bias[n] (fp32, may be NULL), Relu if asked;
  * a is [m][k], b is [n][k], both e4m3.  The sums of a block are the tensor
  * cores', over at most 128 products; blocks are scaled and added in fp32, and y
- * is rounded once.  a and b on 16-byte boundaries with row strides that are
+ * is rounded once.  The product of the two scales is formed first: one below
+ * 2^-126 has fewer bits, one past fp32's range is infinite.  a and b on 16-byte boundaries with row strides that are
  * multiples of 16 run on the tensor cores, others on the CUDA cores (slower,
  * same formula). */
 ONNXB200_API int onnxb200_matmul_blocks(onnxb200_handle* h, const onnxb200_matmul_blocks_desc* d,

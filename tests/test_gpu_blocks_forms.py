@@ -189,3 +189,16 @@ def test_norm_into_the_type_of_the_weight_writes_nothing_else(handle, cols):
         rest = y.clone()
         rest[1:-1, off:off + cols] = 3.0
         assert (rest == 3.0).all()
+
+
+@pytest.mark.parametrize("cols", [256, 1001, 6001])
+def test_norm_past_the_range_of_its_sum(ob, ctx, cols):
+    """A finite row whose sum of squares passes fp32's range gives zeros; with epsilon 0 one whose squares
+    vanish gives values that are not finite.  Each row by itself."""
+    x, w = tb.normal((4, cols), 1), tb.normal((cols,), 2)
+    x[1] *= 1e25
+    x[2] = 1e-30
+    y = ob.RMSNormalization(epsilon=0.0).compute([x, w], ctx)[0]
+    assert (y[1] == 0).all() and not torch.isfinite(y[2]).any()
+    ref = tb.norm_ref(x[[0, 3]], None, w, 0.0)[1]
+    assert ((y[[0, 3]].double() - ref).abs() <= ref.abs() * 39 * U * (1 + 2 ** -10)).all()
