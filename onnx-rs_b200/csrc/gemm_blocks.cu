@@ -39,7 +39,8 @@ __device__ __forceinline__ bool elect_one() {
 // ---------------------------------------------------------------- CUDA cores
 // Operands that TMA cannot read (row strides or pointers off the 16-byte grid):
 // 64 x 64 outputs per block, 4 x 4 per thread; the products of a block of 128
-// k's are summed in fp32, then scaled and added to the total.
+// k's are summed in fp32, then scaled and added to the total.  2048 x 2048 x 2049: 762
+// us, 22.6 TFLOP/s.
 template <typename T>
 __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlocksArgs p) {
   __shared__ float sa[32][65], sb[32][65];
@@ -99,8 +100,8 @@ __global__ void __launch_bounds__(256) matmul_blocks_simt_kernel(const MatmulBlo
 // flight; a is turned into fp16 (exact) once per block, and products are fused into
 // fp32 sums of 16, which are scaled and added.  The mixed fp16 -> fp32 fused
 // multiply-adds run at a quarter of the fp32 rate: 1 x 4096 x 4096 takes 6.7 us (17
-// MB; 8.1 in the kernel for few rows), 1 x 8192 x 8192 15.4 us (4.4 TB/s), 2 x 4096 x
-// 4096 8.3 us, and four rows 10.9, more than below.
+// MB; 8.1 in the kernel for few rows), 1 x 8192 x 8192 15.0 us (4.5 TB/s), 2 x 4096 x
+// 4096 8.2 us, and four rows 10.9, more than below.
 constexpr int kVecWarps = 8, kVecRows = 2, kVecUnroll = 4;
 template <typename T, int M>
 __global__ void __launch_bounds__(kVecWarps * 32) matmul_blocks_vec_kernel(const MatmulBlocksArgs p) {
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kVecWarps * 32) matmul_blocks_vec_kernel(const
 // The k range is split over the CTAs of a cluster; each leaves its partial sums in
 // shared memory, and the sums are joined in rank order over distributed shared
 // memory: one launch, no workspace, the same bits every time.  Bound by HBM with
-// many weights (16 x 14336 x 4096, 59 MB: 15.1 us, 3.9 TB/s), by the start of its
+// many weights (16 x 14336 x 4096, 59 MB: 15.0 us, 3.9 TB/s), by the start of its
 // CTAs and the join with few (16 x 4096 x 4096: 8.7 us, of which 2.6 are bytes).
 template <int BN>
 struct RowsLayout {
@@ -443,10 +444,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 // instead of 64 8192^3 took 523 instead of 503 us, with the next block's first columns
 // loaded under the last additions 527 to 600 (register moves), with sixteen warps and
 // half the totals each 580 (spills); a second warp to issue the MMAs changed nothing.
-// Run without a pause (1.24 to 1.5 GHz): 8192^3 bf16 508 us, 2.16 PFLOP/s; 4096^3 72
-// us; 8192 x 8192 x 1024 80 us (its tiles' output is a sixth); after idle, at higher
-// clocks, 8192^3 435 us.  200 x 8192 x 4096 (256 x 128 tiles, 36 MB) 15 us, its loop
-// at 4.7 TB/s.
+// Run without a pause (1.16 to 1.5 GHz under the power cap): 8192^3 bf16 500 to 530 us,
+// 2.07 to 2.2 PFLOP/s; 4096^3 70 to 73 us; 8192 x 8192 x 1024 80 to 82 us (its tiles'
+// output is a sixth); after idle, at higher clocks, 8192^3 435 to 458 us, 4096^3 62.  200
+// x 8192 x 4096 (256 x 128 tiles, 36 MB) 15 us, its loop at 4.7 TB/s.
 //
 // 8 epilogue warps, then a warpgroup with the TMA, MMA and scale warps.  Launched
 // with 168 registers a thread (384 x 168 = 64512), split as 208 for the totals and

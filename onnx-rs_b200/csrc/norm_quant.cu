@@ -149,8 +149,9 @@ __device__ __forceinline__ bool writes_scale() {
 // before the row's one reduction (a shuffle and a barrier).  Bound by HBM with
 // several blocks per SM taking turns; blocks that walk rows with the next two rows
 // copied ahead were slower (107 against 84 us then: fewer blocks, and the same chain
-// of reductions).  8192 x 8192 bf16 with residual and e4m3 output (470 MB): 74 us,
-// 6.3 TB/s; one row of 4096 2.8 us.
+// of reductions).  8192 x 8192 bf16 with residual and e4m3 output (470 MB): 73 us,
+// 6.4 TB/s (run without a pause, at 1.6 GHz under the power cap, 78 to 80); one row of
+// 4096 2.6 to 2.9 us.
 template <typename T, typename W, int CH, bool WARP = false>
 __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, CH == 4 && sizeof(T) == 2 ? (WARP ? 4 : 2) : 1)
     rmsnorm_vec_kernel(const RmsNormArgs p) {
@@ -258,8 +259,8 @@ __global__ void __launch_bounds__(WARP ? 256 : CH == 4 ? 512 : 1024, CH == 4 && 
 // Any alignment, up to 4096 columns: one row per thread block, blocks of 128 columns
 // dealt to its warps (NB each, four columns a lane), all elements of x, the residual
 // and the weight on their way before the first is used; h stays in registers.  Bound
-// by its element accesses: 4096 x 1001 fp16 with residual and e4m3 output (29 MB)
-// 13.7 us, fp32 without (33 MB) 9.4 us.
+// by instructions, an element each (80% of the issue slots): 4096 x 1001 fp16 with
+// residual and e4m3 output (29 MB) 13.7 us, fp32 without (33 MB) 9.4 us.
 constexpr int kRowThreads = 512;
 template <typename T, typename W, int NB>
 __global__ void __launch_bounds__(kRowThreads, NB == 1 ? 4 : 2) rmsnorm_elem_kernel(const RmsNormArgs p) {
@@ -355,7 +356,10 @@ __global__ void __launch_bounds__(kRowThreads, NB == 1 ? 4 : 2) rmsnorm_elem_ker
 }
 
 // Any alignment and width: one row per block, the row's fp32 sum x + residual held
-// in shared memory.
+// in shared memory.  Bound by instructions, an element each (82% of the issue slots):
+// 333 x 5001 fp16 with residual and e4m3 output (12 MB) 8.0 us, 8192 x 8001 bf16 (459
+// MB) 136 to 143 us; aligned rows of more than 16384 columns take it too (1024 x 20000
+// bf16 64 us, 2.2 TB/s).
 template <typename T, typename W>
 __global__ void __launch_bounds__(kRowThreads) rmsnorm_row_kernel(const RmsNormArgs p) {
   extern __shared__ float row[];
@@ -421,8 +425,8 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_row_kernel(const RmsNormA
 
 // block_rows = 1, aligned rows: a warp takes UNROLL x 256 columns of a row, eight
 // per lane and vector (2 or 4 KB a warp), all loads in flight before the first is used; 16 lanes
-// share a block's scale.  Bound by HBM: 8192 x 4096 fp32 (168 MB) in 27.1 us, 6.2 TB/s;
-// 8192 x 8192 bf16 in 32.8 us, 6.1 TB/s.
+// share a block's scale.  Bound by HBM: 8192 x 4096 fp32 (168 MB) in 27.3 us, 6.2 TB/s;
+// 8192 x 8192 bf16 in 32.8 us, 6.1 TB/s (34.7 run without a pause, at 1.75 GHz).
 constexpr int kQuantUnroll = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_row_vec_kernel(const QuantizeArgs p, unsigned segments, unsigned units) {
@@ -449,7 +453,9 @@ __global__ void __launch_bounds__(256) quantize_row_vec_kernel(const QuantizeArg
   }
 }
 
-// block_rows = 1, any alignment: one warp per block of 128 columns of a row.
+// block_rows = 1, any alignment: one warp per block of 128 columns of a row.  Bound by
+// instructions, an element each (81% of the issue slots): 4096 x 4099 bf16 (50 MB) and
+// fp32 (84 MB) 28 us.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_row_kernel(const QuantizeArgs p, unsigned cb, unsigned units) {
   pdl_begin();
@@ -489,7 +495,7 @@ __device__ __forceinline__ float block_max_nan(float v) {
 
 // block_rows = 128, aligned rows: one thread block per block of 128 x 128, which it
 // reads once (8 vectors of 8 columns per thread) and keeps in registers.  8192 x 8192
-// fp32 51.3 us (6.5 TB/s), bf16 34.6 us (5.8 TB/s).
+// fp32 51.3 us (6.5 TB/s), bf16 34.6 us (5.8 TB/s); 52.3 and 35.6 run without a pause.
 template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) quantize_tile_vec_kernel(const QuantizeArgs p, unsigned cb) {
   pdl_begin();
@@ -613,8 +619,8 @@ int rmsnorm_launch(const RmsNormArgs& a, int num_sms, cudaStream_t st) {
       }
       // With rows enough to fill the GPU: a warp a row up to 1024 columns (8192 x 128
       // bf16: 3.3 us against 10.0 with a block a row), then few threads with more
-      // loads in flight each and cheaper reductions (8192 x 2048: 20.9 us with 128
-      // threads, 23.2 with 256).  Otherwise as many threads as there are vectors.
+      // loads in flight each and cheaper reductions (8192 x 2048 with residual and e4m3
+      // output: 20.9 us with 128 threads, 23.2 with 256).  Otherwise as many threads as there are vectors.
       const int n8 = a.cols / 8;
       const bool many = a.rows > 2 * num_sms;
       if (many && n8 <= 128) {

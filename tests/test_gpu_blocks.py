@@ -1,8 +1,7 @@
 """GPU tests of the 8-bit linear path against plain forms in 64 bits.
 
 Tolerances count roundings.  u = 2^-24 is half a step of fp32, h(t) half a step
-of the output's type (bf16 2^-9 relative to the leading bit, written 2^-8 / 2 *
-2 below as torch.finfo(t).eps / 2).
+of the output's type relative to the value (torch.finfo(t).eps / 2: bf16 2^-8).
 
 rmsnorm: h = x + r is one rounding; the sum of squares adds at most ceil(cols /
 256) + 16 roundings in a row, of which the square root passes half; division,
